@@ -24,36 +24,36 @@ STRIDE = 32                    # staging rows of a lane
 def listed():
     return [
         # one decode step of eight long requests: one page entry at most is new per request, latency is all
-        {"name": "tables, 8 requests, one token each", "op": "tables", "lanes": 8, "pages": 1024, "known": True, "rows": 1},
+        {"name": "tables 8 requests one token each", "op": "tables", "lanes": 8, "pages": 1024, "known": True, "rows": 1},
         # every table of a full batch built anew, verify windows of up to 16 rows
-        {"name": "tables, 1024 requests anew", "op": "tables", "lanes": 1024, "pages": 4096, "known": False, "rows": 16},
+        {"name": "tables 1024 requests anew", "op": "tables", "lanes": 1024, "pages": 4096, "known": False, "rows": 16},
         # 32 requests forked from one 8K-token prefix (the prefix-sharing configuration of the benchmark)
-        {"name": "groups, 32 forks of 8K", "op": "groups", "lanes": 32, "prompts": 1, "pages": 273},
+        {"name": "groups 32 forks of 8K", "op": "groups", "lanes": 32, "prompts": 1, "pages": 273},
         # a large batch over 24 system prompts of different lengths
-        {"name": "groups, 1024 requests of 24 prompts", "op": "groups", "lanes": 1024, "prompts": 24, "pages": 1000},
+        {"name": "groups 1024 requests of 24 prompts", "op": "groups", "lanes": 1024, "prompts": 24, "pages": 1000},
         # best-of-four sampling of one 2K-token prompt
-        {"name": "shared, int8, 4 x 2K", "op": "shared", "format": "int8", "lanes": 4, "groups": 1, "prefix": 2048, "suffix": 100,
+        {"name": "shared int8 4 x 2K", "op": "shared", "format": "int8", "lanes": 4, "groups": 1, "prefix": 2048, "suffix": 100,
          "loose": 0, "softcap": 0.0, "slopes": False},
         # 32 requests over one 8K-token prefix, each up to 512 tokens into its own text
-        {"name": "shared, int4, 32 x 8K", "op": "shared", "format": "int4", "lanes": 32, "groups": 1, "prefix": 8192, "suffix": 512,
+        {"name": "shared int4 32 x 8K", "op": "shared", "format": "int4", "lanes": 32, "groups": 1, "prefix": 8192, "suffix": 512,
          "loose": 0, "softcap": 0.0, "slopes": False},
         # a large batch over one 32K-token document
-        {"name": "shared, int4, 256 x 32K", "op": "shared", "format": "int4", "lanes": 256, "groups": 1, "prefix": 32768, "suffix": 1024,
+        {"name": "shared int4 256 x 32K", "op": "shared", "format": "int4", "lanes": 256, "groups": 1, "prefix": 32768, "suffix": 1024,
          "loose": 0, "softcap": 0.0, "slopes": False},
         # one short request of a bf16 pool
-        {"name": "decode, bf16, 1 x 100, capped", "op": "decode", "format": "bf16", "lanes": 1, "context": 100, "ragged": False,
+        {"name": "decode bf16 1 x 100 capped", "op": "decode", "format": "bf16", "lanes": 1, "context": 100, "ragged": False,
          "softcap": 30.0, "window": 0, "sinks": 0, "slopes": False},
         # a full-attention layer with capped scores, 32 x 16K (the format sweep's size)
-        {"name": "decode, int4, 32 x 16K, capped", "op": "decode", "format": "int4", "lanes": 32, "context": 16384, "ragged": False,
+        {"name": "decode int4 32 x 16K capped", "op": "decode", "format": "int4", "lanes": 32, "context": 16384, "ragged": False,
          "softcap": 50.0, "window": 0, "sinks": 0, "slopes": False},
         # a sliding-window layer with sink tokens and a distance bias, ragged requests of up to 16K tokens
-        {"name": "decode, fp8, 64 x 16K, window 4096", "op": "decode", "format": "fp8", "lanes": 64, "context": 16384, "ragged": True,
+        {"name": "decode fp8 64 x 16K window 4096", "op": "decode", "format": "fp8", "lanes": 64, "context": 16384, "ragged": True,
          "softcap": 0.0, "window": 4096, "sinks": 4, "slopes": True},
         # a 16-row verify window over long capped layers
-        {"name": "verify, int4, 4 x 32K, capped", "op": "verify", "format": "int4", "lanes": 4, "context": 32768, "rows": 16, "capacity": 16,
+        {"name": "verify int4 4 x 32K capped", "op": "verify", "format": "int4", "lanes": 4, "context": 32768, "rows": 16, "capacity": 16,
          "softcap": 50.0, "window": 0, "sinks": 0, "slopes": False},
         # a whole prefill chunk of a sliding-window layer
-        {"name": "prefill, int8, 2048 rows over 6K, window 4096", "op": "prefill", "format": "int8", "context": 6144, "rows": 2048,
+        {"name": "prefill int8 2048 rows over 6K window 4096", "op": "prefill", "format": "int8", "context": 6144, "rows": 2048,
          "softcap": 0.0, "window": 4096, "sinks": 4, "slopes": True},
     ]
 
