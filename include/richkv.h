@@ -140,6 +140,18 @@ int rk_attention_prefill_split_tc(const void *window, uint32_t format, uint32_t 
                                   uint32_t head_dim, const void *queries, float *partials, float *statistics,
                                   const rk_page_entry *table, const rk_prefill_params *params, uint32_t *status,
                                   void *stream);
+/* No counterparts in the reference. The two calls above with a score shape (rk_score_shape): chain windows of 8 or 16
+ * rows and prefill tiles, every format; scratch, split counts and merges are theirs. A window's CTA reads only the pages
+ * with a token that one of its rows sees; the key and value rows of those tokens have to be finite. */
+int rk_attention_verify_split_shaped(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,
+                                     uint32_t head_dim, uint32_t lanes, uint32_t row_capacity, uint32_t grid_splits,
+                                     const void *queries, float *partials, float *statistics,
+                                     const rk_page_entry *const *tables, const rk_verify_params *lane_params,
+                                     rk_kv_layer layer, const rk_score_shape *shape, uint32_t *status, void *stream);
+int rk_attention_prefill_split_shaped(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,
+                                      uint32_t head_dim, const void *queries, float *partials, float *statistics,
+                                      const rk_page_entry *table, const rk_prefill_params *params,
+                                      const rk_score_shape *shape, uint32_t *status, void *stream);
 /* Test hook of the window kernel's timeout path, no counterpart in the reference: rk_attention_verify_split_tc
  * (chain masks) whose waits give up after `spin_limit` polls (at most 2^20) and whose TMA warp never streams the
  * last `withheld_groups` 64-token groups of each split. `status` turns non-zero, tensor memory is released and
@@ -154,6 +166,39 @@ int rk_attention_decode(const void *window, const rk_decode_plan *plan, uint32_t
                         void *output, float *output_f32, float *partials, float *statistics,
                         uint32_t *descriptors, const rk_page_entry *const *tables,
                         const rk_verify_params *lane_params, rk_kv_layer layer, void *stream);
+/* No counterpart in the reference. rk_attention_decode with a score shape (rk_score_shape): only the pages with a token
+ * that the row sees are read. Plan, scratch and status word as for rk_attention_decode. */
+int rk_attention_decode_shaped(const void *window, const rk_decode_plan *plan, uint32_t format, const void *queries,
+                               void *output, float *output_f32, float *partials, float *statistics,
+                               uint32_t *descriptors, const rk_page_entry *const *tables,
+                               const rk_verify_params *lane_params, rk_kv_layer layer, const rk_score_shape *shape,
+                               void *stream);
+/* No counterpart in the reference. rk_attention_decode for a batch in which groups of lanes share the first pages of
+ * their tables: the pages a group shares are read once for all of its lanes, whose query rows are the M side of a tcgen05
+ * contraction; what a lane has behind them streams as in rk_attention_decode; one merge joins both. lane_groups and
+ * group_pages are device arrays of one word per lane, as rk_prefix_groups leaves them: lane l belongs to group
+ * lane_groups[l] (a number below `lanes`; anything else: no group) and group g shares its first group_pages[g] pages, which
+ * are the same in every member's table and full of tokens that every member has committed. `shape` may be null. Scratch
+ * is sized by the plan; the caller zeroes buffers->descriptors once, and its status word (rk_attention_decode_status
+ * with &plan->decode) covers both kernels. At most 1 024 lanes. */
+typedef struct rk_shared_plan {
+  rk_decode_plan decode;
+  uint32_t prefix_ctas, reserved;
+  uint64_t prefix_partials_bytes, prefix_statistics_bytes, prefix_descriptor_bytes;
+} rk_shared_plan;
+typedef struct rk_shared_buffers {
+  float *partials, *statistics; /* plan->decode's */
+  uint32_t *descriptors;
+  float *prefix_partials, *prefix_statistics;
+  uint32_t *prefix_descriptors;
+} rk_shared_buffers;
+int rk_shared_plan_make(uint32_t format, uint32_t kv_heads, uint32_t query_heads, uint32_t head_dim, uint32_t lanes,
+                        uint32_t ctas, rk_shared_plan *plan);
+int rk_attention_decode_shared(const void *window, const rk_shared_plan *plan, uint32_t format, const void *queries,
+                               void *output, float *output_f32, const rk_shared_buffers *buffers,
+                               const rk_page_entry *const *tables, const rk_verify_params *lane_params,
+                               rk_kv_layer layer, const uint32_t *lane_groups, const uint32_t *group_pages,
+                               const rk_score_shape *shape, void *stream);
 /* Sequence split of one long context over several GPUs (new here; the reference is single-GPU, its
  * split merge paged_attention_tile.h:362-404 is the combine). Each rank attends the pages it holds and
  * leaves {max, sum, un-normalised output} per (lane, query head) in `triples`
@@ -241,6 +286,32 @@ int rk_session_step_host(void *session, uint32_t layer, const void *q_host, cons
 int rk_session_finish_host(void *session, void *stream);
 int rk_session_status(void *session, void *stream);
 
+/* ---- a step's tables, built on the GPU -------------------------------------------------------------- */
+/* The device-side counterpart of kv::PageStorage::writeEntries (PageStorage.mm:127-141) for a whole batch, with the
+ * parameter blocks the host would upload. Inputs in device memory, per lane: its pages page_ids[page_offsets[l] ..
+ * page_offsets[l + 1]), its committed tokens and the `rows` this step appends (0: idle). Written: entries [lane][table_pages]
+ * for the pages that committed + rows tokens need, from known_pages[l] on (null: from 0; entries before it and behind the
+ * last needed page stay as they are); the parameter blocks of rk_store_verify and of the decode / verify kernels (their kv
+ * fields are zero: the layer is a launch argument there); row_offsets [lanes + 1], the running sum of the rows; and
+ * row_slots [row_offsets[lanes]], each new row's place page id * 32 + token in page. `tables` stays the caller's: the
+ * address of each lane's row of `entries`. A lane that asks for more rows than row_capacity, more tokens than a sequence
+ * may have, more pages than it names or the table holds, or names a page past page_count is made idle (no live rows: every
+ * kernel skips it; its slots are all ones) and raises the sticky `status` word. Every page named has to lie in an extent
+ * that the pool holds. At most 1 024 lanes; row_slots takes lanes * row_capacity words. */
+int rk_step_tables(const rk_step_pool *pool, uint32_t lanes, uint32_t table_pages, uint32_t row_capacity,
+                   uint32_t split_count, float score_scale, const uint32_t *page_ids, const uint32_t *page_offsets,
+                   const uint32_t *committed, const uint32_t *rows, const uint32_t *known_pages,
+                   rk_page_entry *entries, rk_chunk_params *chunk_params, rk_verify_params *verify_params,
+                   uint32_t *row_offsets, uint64_t *row_slots, uint32_t *status, void *stream);
+/* Which lanes share how long a prefix, from their tables (equal entries are the same page; only pages full on every side
+ * count). Lanes are gathered under the lowest lane that has their first page; of those, the ones that share the p pages
+ * for which (lanes - 1) * p is largest (ties: the larger p) become a group, if there are at least minimum_lanes (>= 2) of
+ * them and p >= minimum_pages. lane_groups[l] = the group's lowest lane, or RK_NO_GROUP; group_pages[l] = p at a group's
+ * lowest lane, 0 elsewhere. Both [lanes], device memory. At most 1 024 lanes. */
+int rk_prefix_groups(uint32_t lanes, const rk_page_entry *const *tables, const rk_verify_params *lane_params,
+                     uint32_t minimum_lanes, uint32_t minimum_pages, uint32_t *lane_groups, uint32_t *group_pages,
+                     void *stream);
+
 /* ---- page moves --------------------------------------------------------------------------------- */
 /* kv::ExtentStorage::copyPages (runtime/ops/PagedKv.hpp:70-75, PageStorage.mm:95-114) on table entries:
  * every tensor of every layer of from_entries[i] onto to_entries[i]. Also the copy-on-write fork. */
@@ -275,6 +346,8 @@ int rk_storage_is_allocated(const void *storage, uint32_t page);
 void rk_storage_window(const void *storage, uint64_t *base, uint64_t *bytes);
 uint32_t rk_storage_layers(const void *storage, rk_kv_layer *out, uint32_t capacity);
 rk_page_entry rk_storage_entry(const void *storage, uint32_t page);
+/* Where the storage's pages lie, for rk_step_tables. The geometry is fixed: extents come and go in place. */
+void rk_storage_step_pool(const void *storage, rk_step_pool *pool);
 int rk_storage_read_extent(const void *storage, uint32_t extent, uint64_t offset, void *host, uint64_t bytes);
 int rk_storage_write_extent(void *storage, uint32_t extent, uint64_t offset, const void *host, uint64_t bytes);
 /* PageStorage::writeEntries (PageStorage.mm:127-141) into a device table. */

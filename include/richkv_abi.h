@@ -95,6 +95,28 @@ typedef struct rk_verify_params {
   float score_scale; /* 0 selects 1/sqrt(head_dim) */
 } rk_verify_params;
 
+/* What a score goes through before the softmax (no counterpart in the reference). A row at position p sees token t when
+ * t <= p and (window == 0 or p - t < window or t < sink_tokens); its score is scale * q.k, then softcap * tanh(score /
+ * softcap) where softcap > 0, then minus slopes[query head] * (p - t) where slopes is given (device memory, one fp32 per
+ * query head). sink_tokens counts only beside a window. */
+typedef struct rk_score_shape {
+  float softcap;       /* 0: none */
+  uint32_t window;     /* 0: none */
+  uint32_t sink_tokens;
+  uint32_t reserved;   /* 0 */
+  const float *slopes; /* null: none */
+} rk_score_shape;
+
+/* Where page ids lie (rk_storage_step_pool): page id i is page i % extent_pages of the extent at
+ * base + i / extent_pages * extent_stride. */
+typedef struct rk_step_pool {
+  uint64_t base, extent_stride;
+  uint32_t extent_pages, page_count;
+} rk_step_pool;
+
+/* A lane that belongs to no group of lanes with a shared prefix. */
+#define RK_NO_GROUP 0xffffffffu
+
 /* A page whose content goes to another page (PagedKv.hpp:49-53). */
 typedef struct rk_page_copy {
   uint32_t from;
@@ -107,6 +129,8 @@ static_assert(sizeof(rk_chunk_params) == 24, "chunk store parameters are 24 byte
 static_assert(sizeof(rk_prefill_params) == 32, "prefill parameters are 32 bytes");
 static_assert(sizeof(rk_verify_params) == 36, "verify parameters are 36 bytes");
 static_assert(sizeof(rk_page_copy) == 8, "page copy is 8 bytes");
+static_assert(sizeof(rk_score_shape) == 24 && offsetof(rk_score_shape, slopes) == 16, "score shape is 24 bytes");
+static_assert(sizeof(rk_step_pool) == 24, "step pool is 24 bytes");
 static_assert(offsetof(rk_chunk_params, kv) == 16, "chunk kv offset");
 static_assert(offsetof(rk_prefill_params, kv) == 16 &&
                   offsetof(rk_prefill_params, split_count) == 24 &&

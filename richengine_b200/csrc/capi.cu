@@ -296,6 +296,10 @@ extern "C" void rk_storage_window(const void *storage, uint64_t *base, uint64_t 
   *base = uint64_t(s->base);
   *bytes = s->reserved;
 }
+extern "C" void rk_storage_step_pool(const void *storage, rk_step_pool *pool) {
+  const auto *s = static_cast<const Storage *>(storage);
+  *pool = rk_step_pool{uint64_t(s->base), s->extent_stride, s->extent_pages, s->page_count};
+}
 extern "C" uint32_t rk_storage_layers(const void *storage, rk_kv_layer *out, uint32_t capacity) {
   const auto *s = static_cast<const Storage *>(storage);
   for (uint32_t i = 0; i < s->layers && i < capacity; ++i) out[i] = s->places[i];

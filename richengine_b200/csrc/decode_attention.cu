@@ -30,6 +30,8 @@
 //  * A CTA's last segment is folded in the (then idle) ring to one partial per KV head before it leaves the SM; the
 //    merge kernel that follows (a programmatic dependent launch) combines a lane's partials in segment order.
 #include "common.cuh"
+#include "decode_partials.cuh"
+#include "score_shape.cuh"
 #include "window.cuh"
 
 #include <cuda.h>
@@ -70,6 +72,7 @@ constexpr uint32_t kSpinLimit = 1u << 20; // polls of ~100 ns: a wait gives up a
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 static_assert(kStageBytes % 1024 == 0, "stages keep the 1 KiB swizzle alignment");
+static_assert(kPageWarps == kDecodeSlotsPerSegment && kKvHeads == kDecodeHeads, "the partials' layout");
 
 struct DecodeArgs {
   const uint16_t *queries;
@@ -84,6 +87,26 @@ struct DecodeArgs {
   uint32_t *status;     // sticky device status word: set when a bounded wait ran out, cleared by the status readers
   uint32_t spin_limit;  // polls a wait may take (kSpinLimit in production; the timeout probe passes a few thousand)
   uint32_t withheld;    // timeout probe only: the producer never streams the last `withheld` pages of its range
+  // shaped launches (kShaped) only
+  ShapeArgs shape;
+  const uint32_t *lane_groups = nullptr, *group_pages = nullptr; // a lane leaves the first group_pages[its group] pages out
+};
+
+// The pages a shaped lane reads: the shape's list without the pages of its group's shared prefix.
+__device__ __forceinline__ PageList lane_list(const DecodeArgs &args, uint32_t l, uint32_t committed) {
+  uint32_t skip = 0;
+  if (args.lane_groups) {
+    const uint32_t group = args.lane_groups[l];
+    if (group < args.lanes) skip = args.group_pages[group];
+  }
+  return PageList::make(committed, committed, skip, args.shape);
+}
+// What the shaped softmax needs beside the scores of a page.
+struct ShapedPage {
+  float cap, cap_inverse; // in the log2 domain; 0: no cap
+  float slope[2];         // of this thread's two query heads, in the log2 domain
+  float distance;         // the row's position minus the page's first token
+  uint32_t seen;          // bit t: token t of the page is seen
 };
 
 __device__ __forceinline__ uint32_t smem_address(const void *p) { return uint32_t(__cvta_generic_to_shared(p)); }
@@ -281,11 +304,13 @@ __device__ void exclusive_scan(uint32_t *values, uint32_t n, uint32_t *scratch) 
 
 // Online softmax of one page for this lane's 4 tokens x 2 query heads, and the fp16 probability
 // fragments (B operand of O^T += V^T.P^T). Masked = the page holds tokens past the visible ones.
-template <bool Masked, bool Wide = false, bool Ride = false>
+// Shaped: the mask is shaped->seen instead of the tokens below `valid`, and every score passes the cap and the bias.
+template <bool Masked, bool Wide = false, bool Ride = false, bool Shaped = false>
 __device__ __forceinline__ void page_softmax(const float (&sacc)[2][2][4], const float (&hfac)[2],
                                              const float (&negoff)[2], uint32_t scales, uint32_t r3g,
                                              uint32_t valid, float (&m)[2], float (&l_sum)[2], float (&o)[16][4],
-                                             uint32_t (&pb_frag)[2][2], uint32_t (*pb_low)[2] = nullptr, float *psum = nullptr) {
+                                             uint32_t (&pb_frag)[2][2], uint32_t (*pb_low)[2] = nullptr, float *psum = nullptr,
+                                             const ShapedPage *shaped = nullptr) {
   float s2[2][2][2], lv[2][2];
   float local_max[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -295,13 +320,18 @@ __device__ __forceinline__ void page_softmax(const float (&sacc)[2][2][4], const
       const uint32_t token = 16 * mt + 8 * half + r3g;
       const float ks = load_shared_f32(scales + token * 4);
       const float vs = load_shared_f32(scales + kScaleBytes + token * 4);
-      const bool live = !Masked || token < valid;
+      const bool live = !Masked || (Shaped ? (shaped->seen >> token) & 1u : token < valid);
       lv[mt][half] = live ? log2_fast(vs) : -INFINITY; // a zero value row weighs nothing
       const float floor_lv = live ? fmaxf(lv[mt][half], -40.0f) : -INFINITY;
 #pragma unroll
       for (uint32_t j = 0; j < 2; ++j) {
         const float acc = sacc[mt][0][half * 2 + j] + sacc[mt][1][half * 2 + j];
-        const float score = live ? fmaf(acc, hfac[j], negoff[j]) * ks : -INFINITY;
+        float value = fmaf(acc, hfac[j], negoff[j]) * ks;
+        if (Shaped) {
+          if (shaped->cap > 0.0f) value = soft_cap(value, shaped->cap, shaped->cap_inverse);
+          value = fmaf(shaped->slope[j], float(token) - shaped->distance, value);
+        }
+        const float score = live ? value : -INFINITY;
         s2[mt][half][j] = score;
         local_max[j] = fmaxf(local_max[j], score + floor_lv);
       }
@@ -370,13 +400,14 @@ __device__ __forceinline__ void dependents_may_launch() { asm volatile("griddepc
 // changes here: the int4 loop runs at the edge of what the SM issues, and its schedule moved by 2 % with unrelated
 // edits of a prologue compiled into the same body. Every thread of the CTA calls it; an empty range comes back as
 // range_begin == range_end.
+template <bool kShaped>
 __device__ __noinline__ void cut_ranges(Shared &sh, const DecodeArgs &args, uint32_t switch_pages) {
   const uint32_t tid = threadIdx.x, lanes = args.lanes, cta = blockIdx.x;
   for (uint32_t i = tid; i < lanes; i += kThreads) {
     rk_verify_params p = args.lane_params[i];
     p.kv = args.layer;
     const bool valid = rk_verify_contract_valid(&p) && p.active_rows == 1 && p.row_capacity == 1;
-    sh.lane_start[i] = valid ? rk_pages_for(p.committed_tokens + 1) : 0;
+    sh.lane_start[i] = !valid ? 0 : kShaped ? lane_list(args, i, p.committed_tokens).count : rk_pages_for(p.committed_tokens + 1);
   }
   if (tid == 0) { sh.error = 0; sh.range_begin = sh.range_end = sh.first_lane = 0; }
   __syncthreads();
@@ -384,6 +415,10 @@ __device__ __noinline__ void cut_ranges(Shared &sh, const DecodeArgs &args, uint
   const uint64_t total_pages = sh.lane_start[lanes];
   // Never more ranges than pages, so every range between a lane's first and last is non-empty.
   const uint32_t ctas = uint32_t(min(uint64_t(gridDim.x), total_pages));
+  if (kShaped && !ctas && cta == 0) { // every lane lies inside its group's prefix: no lane has a segment
+    dependency_wait();
+    for (uint32_t i = tid; i < lanes; i += kThreads) args.descriptors[2 * i] = args.descriptors[2 * i + 1] = 0;
+  }
   if (cta >= ctas) return; // the whole CTA: its range stays empty (it never needed its predecessor's results)
   const Cut cut = Cut::make(total_pages, ctas, lanes, switch_pages);
   for (uint32_t i = tid; i < lanes; i += kThreads) {
@@ -462,25 +497,11 @@ __device__ __forceinline__ void fold_and_store(const FoldScratch &fold, uint32_t
     }
   }
 }
-// A lane's descriptor {first segment, segments | last segment holds three slots << 31} -> its partial slots in order.
-struct LaneSlots {
-  uint32_t first, single, slots; // segments [first, first + single) hold one slot each; then up to three of segment first + single
-  __device__ __forceinline__ explicit LaneSlots(uint2 descriptor) {
-    const uint32_t segments = descriptor.y & 0x7fffffffu, triple = descriptor.y >> 31;
-    first = descriptor.x;
-    single = segments - (segments ? triple : 0u);
-    slots = single + (segments - single) * kPageWarps;
-  }
-  __device__ __forceinline__ uint64_t slot(uint32_t t, uint32_t head) const {
-    return t < single ? (uint64_t(first + t) * kKvHeads + head) * kPageWarps
-                      : (uint64_t(first + single) * kKvHeads + head) * kPageWarps + (t - single);
-  }
-};
-
 __device__ __forceinline__ void group_barrier(uint32_t id, uint32_t threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+template <bool kShaped>
 __global__ void __launch_bounds__(kThreads, 1)
 decode_int4_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs args) {
   extern __shared__ uint8_t dynamic_shared[];
@@ -501,7 +522,7 @@ decode_int4_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  cut_ranges(sh, args, kSwitchPages);
+  cut_ranges<kShaped>(sh, args, kSwitchPages);
   const uint32_t range_begin = sh.range_begin, range_end = sh.range_end, first_lane = sh.first_lane;
   if (range_begin >= range_end) return;
   const Cut cut = sh.cut;
@@ -525,17 +546,23 @@ decode_int4_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
       const uint32_t pb = min(range_end, lane_end) - lane_begin;
       if (pb <= pa || lane_end <= range_begin) continue;
       const rk_page_entry *table = upcoming ? upcoming_table : args.tables[l];
-      rk_page_entry next_entry = upcoming ? upcoming_first : table[pa];
+      PageList list;
+      if (kShaped) list = lane_list(args, l, args.lane_params[l].committed_tokens);
+      rk_page_entry next_entry = upcoming ? upcoming_first : table[kShaped ? list.page(pa) : pa];
       // the next lane with pages in this range starts at its page 0
       uint32_t after = l + 1;
       while (after < lanes && sh.lane_start[after + 1] == sh.lane_start[after]) ++after;
       upcoming = after < lanes && sh.lane_start[after] < range_end;
-      if (upcoming) upcoming_table = args.tables[after];
+      uint32_t upcoming_page = 0;
+      if (upcoming) {
+        upcoming_table = args.tables[after];
+        if (kShaped) upcoming_page = lane_list(args, after, args.lane_params[after].committed_tokens).page(0);
+      }
       const uint32_t fetch_at = pa + min(8u, pb - pa - 1);
       for (uint32_t page = pa; ok && unit < issue_limit && page < pb; ++page, ++unit) {
         const rk_page_entry entry = next_entry;
-        if (page + 1 < pb) next_entry = table[page + 1]; // in flight while this page's copies are issued
-        if (upcoming && page == fetch_at) upcoming_first = upcoming_table[0];
+        if (page + 1 < pb) next_entry = table[kShaped ? list.page(page + 1) : page + 1]; // in flight while this page's copies are issued
+        if (upcoming && page == fetch_at) upcoming_first = upcoming_table[kShaped ? upcoming_page : 0];
         const uint32_t index = rk_entry_index(entry);
         const uint64_t region = rk_entry_extent(entry) + args.layer.offset;
         const uint64_t pages = args.layer.extent_pages;
@@ -585,6 +612,16 @@ decode_int4_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
     const rk_verify_params p = args.lane_params[l];
     const uint32_t visible = p.committed_tokens + 1;
     const uint32_t lane_pages = lane_end - lane_begin;
+    PageList list;
+    ShapedPage shaped;
+    if (kShaped) {
+      list = lane_list(args, l, p.committed_tokens);
+      shaped.cap = args.shape.cap;
+      shaped.cap_inverse = args.shape.cap_inverse;
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j)
+        shaped.slope[j] = args.shape.slopes && 2 * c + j < kGroup ? __ldg(args.shape.slopes + head * kGroup + 2 * c + j) * kLog2e : 0.0f;
+    }
 
     // ---- the head's query fragments (B operand of S^T = K.Q^T), shared by its three warps ----
     group_barrier(1 + head, kPageWarps * 32); // every warp of the head is done with the previous lane
@@ -664,7 +701,15 @@ decode_int4_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
       const uint32_t keys = stage + head * kSlabBytes;
       const uint32_t values = stage + kTensorBytes + head * kSlabBytes;
       const uint32_t scales = stage + 2 * kTensorBytes + head * (kPageTokens * 4);
-      const uint32_t valid = page + 1 == lane_pages ? visible - page * kPageTokens : kPageTokens;
+      uint32_t valid = kPageTokens;
+      if (kShaped) { // valid only says whether the page is seen whole
+        const uint32_t base = list.page(page) * kPageTokens;
+        shaped.seen = seen_tokens(base, p.committed_tokens, list.window_first, args.shape.sinks);
+        shaped.distance = float(int32_t(p.committed_tokens - base));
+        if (shaped.seen != 0xffffffffu) valid = 0;
+      } else if (page + 1 == lane_pages) {
+        valid = visible - page * kPageTokens;
+      }
 
       // ---- S^T = K.Q^T : two 16-token tiles, 16 k-steps each --------------------------
       float sacc[2][2][4];
@@ -703,9 +748,9 @@ decode_int4_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
       // ---- online softmax over the page's 32 tokens -------------------------------------
       uint32_t pb_frag[2][2];
       if (valid == kPageTokens)
-        page_softmax<false, false, true>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag, nullptr, psum);
+        page_softmax<false, false, true, kShaped>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag, nullptr, psum, &shaped);
       else
-        page_softmax<true, false, true>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag, nullptr, psum);
+        page_softmax<true, false, true, kShaped>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag, nullptr, psum, &shaped);
 
       // ---- O^T += V^T.P^T : 16 tiles of 16 dims, 2 k-steps of 16 tokens -----------------
 #pragma unroll
@@ -856,7 +901,7 @@ template <bool kFloat8> __device__ __forceinline__ uint32_t value_pair(uint32_t 
   return sub_f16x2(__byte_perm(word ^ 0x80808080u, 0x64646464u, selector), 0x64806480u);
 }
 
-template <bool kFloat8>
+template <bool kFloat8, bool kShaped>
 __global__ void __launch_bounds__(kThreads, 1)
 decode_bytes_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs args) {
   extern __shared__ uint8_t dynamic_shared[];
@@ -877,7 +922,7 @@ decode_bytes_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs a
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  cut_ranges(sh, args, kByteSwitchPages);
+  cut_ranges<kShaped>(sh, args, kByteSwitchPages);
   const uint32_t range_begin = sh.range_begin, range_end = sh.range_end, first_lane = sh.first_lane;
   if (range_begin >= range_end) return;
   const Cut cut = sh.cut;
@@ -896,10 +941,12 @@ decode_bytes_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs a
       const uint32_t pb = min(range_end, lane_end) - lane_begin;
       if (pb <= pa || lane_end <= range_begin) continue;
       const rk_page_entry *table = args.tables[l];
-      rk_page_entry next_entry = table[pa];
+      PageList list;
+      if (kShaped) list = lane_list(args, l, args.lane_params[l].committed_tokens);
+      rk_page_entry next_entry = table[kShaped ? list.page(pa) : pa];
       for (uint32_t page = pa; ok && unit < issue_limit && page < pb; ++page, ++unit) {
         const rk_page_entry entry = next_entry;
-        if (page + 1 < pb) next_entry = table[page + 1]; // in flight while this page's copies are issued
+        if (page + 1 < pb) next_entry = table[kShaped ? list.page(page + 1) : page + 1]; // in flight while this page's copies are issued
         const uint32_t index = rk_entry_index(entry);
         const uint64_t region = rk_entry_extent(entry) + args.layer.offset;
         const uint64_t pages = args.layer.extent_pages;
@@ -955,6 +1002,16 @@ decode_bytes_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs a
     const rk_verify_params p = args.lane_params[l];
     const uint32_t visible = p.committed_tokens + 1;
     const uint32_t lane_pages = lane_end - lane_begin;
+    PageList list;
+    ShapedPage shaped;
+    if (kShaped) {
+      list = lane_list(args, l, p.committed_tokens);
+      shaped.cap = args.shape.cap;
+      shaped.cap_inverse = args.shape.cap_inverse;
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j)
+        shaped.slope[j] = args.shape.slopes && 2 * c + j < kGroup ? __ldg(args.shape.slopes + head * kGroup + 2 * c + j) * kLog2e : 0.0f;
+    }
 
     // ---- the head's query fragments (B operand of S^T = K.Q^T), shared by its three warps ----
     group_barrier(1 + head, kPageWarps * 32); // every warp of the head is done with the previous lane
@@ -1032,7 +1089,15 @@ decode_bytes_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs a
       const uint32_t keys = stage + head * kByteSlabBytes;
       const uint32_t values = stage + kByteTensorBytes + head * kByteSlabBytes;
       const uint32_t scales = stage + 2 * kByteTensorBytes + head * (kPageTokens * 4);
-      const uint32_t valid = page + 1 == lane_pages ? visible - page * kPageTokens : kPageTokens;
+      uint32_t valid = kPageTokens;
+      if (kShaped) { // valid only says whether the page is seen whole
+        const uint32_t base = list.page(page) * kPageTokens;
+        shaped.seen = seen_tokens(base, p.committed_tokens, list.window_first, args.shape.sinks);
+        shaped.distance = float(int32_t(p.committed_tokens - base));
+        if (shaped.seen != 0xffffffffu) valid = 0;
+      } else if (page + 1 == lane_pages) {
+        valid = visible - page * kPageTokens;
+      }
 
       // ---- S^T = K.Q^T : two 16-token tiles, 16 k-steps each --------------------------
       float sacc[2][2][4];
@@ -1070,9 +1135,9 @@ decode_bytes_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs a
       // ---- online softmax over the page's 32 tokens -------------------------------------
       uint32_t pb_frag[2][2];
       if (valid == kPageTokens)
-        page_softmax<false>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag);
+        page_softmax<false, false, false, kShaped>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag, nullptr, nullptr, &shaped);
       else
-        page_softmax<true>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag);
+        page_softmax<true, false, false, kShaped>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag, nullptr, nullptr, &shaped);
 
       if (kFloat8 && valid != kPageTokens) {
         // A lane's last page: stale bytes past the visible tokens may decode to NaN, and a zero weight must meet a
@@ -1082,8 +1147,15 @@ decode_bytes_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs a
         for (uint32_t i = lane; i < kByteSlabBytes / 4; i += 32) {
           const uint32_t row = i >> 5, half = (((i >> 2) & 7u) ^ row) & 1u;
           const uint32_t first_token = 16 * half + 4 * (i & 3u);
-          if (first_token + 4 <= valid) continue;
-          const uint32_t keep = first_token >= valid ? 0u : (1u << (8 * (valid - first_token))) - 1u;
+          uint32_t keep;
+          if (kShaped) { // the four tokens' bits, spread to bytes
+            const uint32_t four = (shaped.seen >> first_token) & 15u;
+            if (four == 15u) continue;
+            keep = ((four * 0x00204081u) & 0x01010101u) * 255u;
+          } else {
+            if (first_token + 4 <= valid) continue;
+            keep = first_token >= valid ? 0u : (1u << (8 * (valid - first_token))) - 1u;
+          }
           const uint32_t word = load_shared_32(values + 4 * i) & keep;
           asm volatile("st.shared.u32 [%0], %1;" ::"r"(values + 4 * i), "r"(word) : "memory");
         }
@@ -1167,6 +1239,7 @@ constexpr uint32_t kWideSlabBytes = 16384; // one head's K (or V) of a page: one
 constexpr uint32_t kWideStageBytes = 2 * kWideSlabBytes;
 static_assert(kWideStages <= kStages, "the barrier arrays hold the stages");
 
+template <bool kShaped>
 __global__ void __launch_bounds__(kThreads, 1)
 decode_bf16_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs args) {
   extern __shared__ uint8_t dynamic_shared[];
@@ -1189,7 +1262,7 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (uint32_t i = tid; i < sizeof(sh.unit_scales) / sizeof(float); i += kThreads) sh.unit_scales[i] = 1.0f;
-  cut_ranges(sh, args, kWideSwitchPages);
+  cut_ranges<kShaped>(sh, args, kWideSwitchPages);
   const uint32_t range_begin = sh.range_begin, range_end = sh.range_end, first_lane = sh.first_lane;
   if (range_begin >= range_end) return;
   const Cut cut = sh.cut;
@@ -1208,10 +1281,12 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
       const uint32_t pb = min(range_end, lane_end) - lane_begin;
       if (pb <= pa || lane_end <= range_begin) continue;
       const rk_page_entry *table = args.tables[l];
-      rk_page_entry next_entry = table[pa];
+      PageList list;
+      if (kShaped) list = lane_list(args, l, args.lane_params[l].committed_tokens);
+      rk_page_entry next_entry = table[kShaped ? list.page(pa) : pa];
       for (uint32_t page = pa; ok && ordinal < issue_limit && page < pb; ++page, ++ordinal) {
         const rk_page_entry entry = next_entry;
-        if (page + 1 < pb) next_entry = table[page + 1]; // in flight while this page's copies are issued
+        if (page + 1 < pb) next_entry = table[kShaped ? list.page(page + 1) : page + 1]; // in flight while this page's copies are issued
         const uint32_t index = rk_entry_index(entry);
         const uint64_t region = rk_entry_extent(entry) + args.layer.offset;
         const uint64_t keys = region + uint64_t(index) * (kKvHeads * kWideSlabBytes);
@@ -1262,6 +1337,16 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
     const rk_verify_params p = args.lane_params[l];
     const uint32_t visible = p.committed_tokens + 1;
     const uint32_t lane_pages = lane_end - lane_begin;
+    PageList list;
+    ShapedPage shaped;
+    if (kShaped) {
+      list = lane_list(args, l, p.committed_tokens);
+      shaped.cap = args.shape.cap;
+      shaped.cap_inverse = args.shape.cap_inverse;
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j)
+        shaped.slope[j] = args.shape.slopes && 2 * c + j < kGroup ? __ldg(args.shape.slopes + head * kGroup + 2 * c + j) * kLog2e : 0.0f;
+    }
 
     // ---- the head's query fragments (B operand of S^T = K.Q^T), shared by its three warps ----
     group_barrier(1 + head, kPageWarps * 32); // every warp of the head is done with the previous lane
@@ -1306,7 +1391,15 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
       }
       const uint32_t keys = ring + slot * kWideStageBytes;
       const uint32_t values = keys + kWideSlabBytes;
-      const uint32_t valid = page + 1 == lane_pages ? visible - page * kPageTokens : kPageTokens;
+      uint32_t valid = kPageTokens;
+      if (kShaped) { // valid only says whether the page is seen whole
+        const uint32_t base = list.page(page) * kPageTokens;
+        shaped.seen = seen_tokens(base, p.committed_tokens, list.window_first, args.shape.sinks);
+        shaped.distance = float(int32_t(p.committed_tokens - base));
+        if (shaped.seen != 0xffffffffu) valid = 0;
+      } else if (page + 1 == lane_pages) {
+        valid = visible - page * kPageTokens;
+      }
 
       // ---- S^T = K.Q^T : two 16-token tiles, 16 k-steps each --------------------------
       float sacc[2][2][4];
@@ -1338,9 +1431,9 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
       // ---- online softmax over the page's 32 tokens -------------------------------------
       uint32_t pb_frag[2][2], pb_low[2][2];
       if (valid == kPageTokens)
-        page_softmax<false, true>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag, pb_low);
+        page_softmax<false, true, false, kShaped>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag, pb_low, nullptr, &shaped);
       else
-        page_softmax<true, true>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag, pb_low);
+        page_softmax<true, true, false, kShaped>(sacc, hfac, negoff, scales, r3g, valid, m, l_sum, o, pb_frag, pb_low, nullptr, &shaped);
 
       // ---- O^T += V^T.P^T : 16 tiles of 16 dims (rows g and g+8 of a tile = dims 16t+g, 16t+8+g), 2 k-steps of 16 tokens
 #pragma unroll
@@ -1349,8 +1442,14 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
         uint32_t low = 0xffffffffu, high = 0xffffffffu;
         if (valid != kPageTokens) { // stale bits past the visible tokens may be NaN: a zero weight must meet a finite value
           const uint32_t token = 16 * s + 2 * c;
-          low = (token < valid ? 0x0000ffffu : 0u) | (token + 1 < valid ? 0xffff0000u : 0u);
-          high = (token + 8 < valid ? 0x0000ffffu : 0u) | (token + 9 < valid ? 0xffff0000u : 0u);
+          if (kShaped) {
+            const uint32_t bits = shaped.seen >> token;
+            low = (bits & 1u ? 0x0000ffffu : 0u) | (bits & 2u ? 0xffff0000u : 0u);
+            high = (bits & 256u ? 0x0000ffffu : 0u) | (bits & 512u ? 0xffff0000u : 0u);
+          } else {
+            low = (token < valid ? 0x0000ffffu : 0u) | (token + 1 < valid ? 0xffff0000u : 0u);
+            high = (token + 8 < valid ? 0x0000ffffu : 0u) | (token + 9 < valid ? 0xffff0000u : 0u);
+          }
         }
 #pragma unroll
         for (uint32_t t = 0; t < 16; ++t) {
@@ -1741,10 +1840,17 @@ int configure_decode_kernel() {
   if (int st = cuda_status(cudaGetDevice(&device), "cudaGetDevice")) return st;
   if (device < 0 || device >= 64) { set_error("device index out of range"); return kInvalid; }
   if (!configured[device].load(std::memory_order_acquire)) {
-    if (int st = cuda_status(cudaFuncSetAttribute(decode_int4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kDecodeSharedBytes)), "decode shared memory")) return st;
-    if (int st = cuda_status(cudaFuncSetAttribute(decode_bytes_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kByteDecodeSharedBytes)), "decode shared memory")) return st;
-    if (int st = cuda_status(cudaFuncSetAttribute(decode_bytes_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kByteDecodeSharedBytes)), "decode shared memory")) return st;
-    if (int st = cuda_status(cudaFuncSetAttribute(decode_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kWideDecodeSharedBytes)), "decode shared memory")) return st;
+    auto allow = [](auto kernel, size_t bytes) {
+      return cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "decode shared memory");
+    };
+    if (int st = allow(decode_int4_kernel<false>, kDecodeSharedBytes)) return st;
+    if (int st = allow(decode_int4_kernel<true>, kDecodeSharedBytes)) return st;
+    if (int st = allow(decode_bytes_kernel<false, false>, kByteDecodeSharedBytes)) return st;
+    if (int st = allow(decode_bytes_kernel<false, true>, kByteDecodeSharedBytes)) return st;
+    if (int st = allow(decode_bytes_kernel<true, false>, kByteDecodeSharedBytes)) return st;
+    if (int st = allow(decode_bytes_kernel<true, true>, kByteDecodeSharedBytes)) return st;
+    if (int st = allow(decode_bf16_kernel<false>, kWideDecodeSharedBytes)) return st;
+    if (int st = allow(decode_bf16_kernel<true>, kWideDecodeSharedBytes)) return st;
     configured[device].store(true, std::memory_order_release);
   }
   return kOk;
@@ -1815,7 +1921,7 @@ static int launch_exchange(uint32_t lanes, cudaStream_t stream, const float *par
 // The streaming kernel of a format on `ctas` CTAs.
 // Launched as a programmatic dependent of whatever precedes it on the stream: its CTAs may be placed while that
 // kernel drains (the kernel waits for its predecessor's writes before it reads anything).
-static int launch_decode(uint32_t format, uint32_t ctas, cudaStream_t s, const Window *w, const DecodeArgs &args) {
+static int launch_decode(uint32_t format, uint32_t ctas, cudaStream_t s, const Window *w, const DecodeArgs &args, bool shaped = false) {
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(ctas);
   config.blockDim = dim3(kThreads);
@@ -1825,12 +1931,26 @@ static int launch_decode(uint32_t format, uint32_t ctas, cudaStream_t s, const W
   attribute.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  cudaError_t error;
-  if (format == RK_FORMAT_INT4) { config.dynamicSmemBytes = kDecodeSharedBytes; error = cudaLaunchKernelEx(&config, decode_int4_kernel, w->int4_map, args); }
-  else if (format == RK_FORMAT_INT8) { config.dynamicSmemBytes = kByteDecodeSharedBytes; error = cudaLaunchKernelEx(&config, decode_bytes_kernel<false>, w->int4_map, args); }
-  else if (format == RK_FORMAT_FP8E4M3) { config.dynamicSmemBytes = kByteDecodeSharedBytes; error = cudaLaunchKernelEx(&config, decode_bytes_kernel<true>, w->int4_map, args); }
-  else { config.dynamicSmemBytes = kWideDecodeSharedBytes; error = cudaLaunchKernelEx(&config, decode_bf16_kernel, w->int4_map, args); }
-  return cuda_status(error, "decode launch");
+  auto launch = [&](auto kernel, size_t shared_bytes) {
+    config.dynamicSmemBytes = shared_bytes;
+    return cuda_status(cudaLaunchKernelEx(&config, kernel, w->int4_map, args), "decode launch");
+  };
+  switch (format) {
+  case RK_FORMAT_INT4: return shaped ? launch(decode_int4_kernel<true>, kDecodeSharedBytes) : launch(decode_int4_kernel<false>, kDecodeSharedBytes);
+  case RK_FORMAT_INT8: return shaped ? launch(decode_bytes_kernel<false, true>, kByteDecodeSharedBytes) : launch(decode_bytes_kernel<false, false>, kByteDecodeSharedBytes);
+  case RK_FORMAT_FP8E4M3: return shaped ? launch(decode_bytes_kernel<true, true>, kByteDecodeSharedBytes) : launch(decode_bytes_kernel<true, false>, kByteDecodeSharedBytes);
+  default: return shaped ? launch(decode_bf16_kernel<true>, kWideDecodeSharedBytes) : launch(decode_bf16_kernel<false>, kWideDecodeSharedBytes);
+  }
+}
+
+int rk::launch_decode_suffix(uint32_t format, const rk_decode_plan &plan, cudaStream_t stream, const Window *window, const void *queries,
+                             float *partials, float *statistics, uint32_t *descriptors, const rk_page_entry *const *tables,
+                             const rk_verify_params *lane_params, rk_kv_layer layer, const ShapeArgs &shape, const uint32_t *lane_groups,
+                             const uint32_t *group_pages) {
+  if (int st = configure_decode_kernel()) return st;
+  const DecodeArgs args{static_cast<const uint16_t *>(queries), partials, statistics, descriptors, tables, lane_params, layer, window->base,
+                        plan.lanes, descriptors + 2 * plan.lanes, kSpinLimit, 0, shape, lane_groups, group_pages};
+  return launch_decode(format, plan.ctas, stream, window, args, true);
 }
 
 extern "C" {
@@ -1895,6 +2015,27 @@ int rk_attention_decode(const void *window, const rk_decode_plan *plan, uint32_t
   DecodeArgs args{static_cast<const uint16_t *>(queries), partials, statistics, descriptors, tables, lane_params, layer, w->base, plan->lanes,
                   descriptors + 2 * plan->lanes, kSpinLimit, 0};
   if (int st = launch_decode(format, plan->ctas, s, w, args)) return st;
+  return launch_merge(plan->lanes, s, partials, statistics, descriptors, static_cast<uint16_t *>(output), output_f32, lane_params, layer, nullptr);
+}
+
+// The same step with a score shape: the streaming kernels list the pages that the row sees (none of the others is read)
+// and pass every score through the shape.
+int rk_attention_decode_shaped(const void *window, const rk_decode_plan *plan, uint32_t format, const void *queries,
+                               void *output, float *output_f32, float *partials, float *statistics, uint32_t *descriptors,
+                               const rk_page_entry *const *tables, const rk_verify_params *lane_params, rk_kv_layer layer,
+                               const rk_score_shape *shape, void *stream) {
+  const auto *w = static_cast<const Window *>(window);
+  ShapeArgs shape_args;
+  if (!w || !plan || !queries || !output || !partials || !statistics || !descriptors || !tables || !lane_params ||
+      !layer.extent_pages || format < RK_FORMAT_INT8 || format > RK_FORMAT_FP8E4M3 || !shape || !shape_arguments(shape, shape_args)) {
+    set_error("rk_attention_decode_shaped: invalid arguments");
+    return kInvalid;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (int st = configure_decode_kernel()) return st;
+  DecodeArgs args{static_cast<const uint16_t *>(queries), partials, statistics, descriptors, tables, lane_params, layer, w->base, plan->lanes,
+                  descriptors + 2 * plan->lanes, kSpinLimit, 0, shape_args};
+  if (int st = launch_decode(format, plan->ctas, s, w, args, true)) return st;
   return launch_merge(plan->lanes, s, partials, statistics, descriptors, static_cast<uint16_t *>(output), output_f32, lane_params, layer, nullptr);
 }
 

@@ -1,0 +1,90 @@
+// score_shape.cuh — what a score goes through between the contraction and the softmax (rk_score_shape): a tanh cap, a
+// bias that falls with the distance, a sliding window with sink tokens; and the pages that such a row reads.
+//
+//   x = scale * q.k            x = cap * tanh(x / cap)  (cap > 0)            x -= slope * (p - t)  (slopes given)
+//   seen(p, t) = t <= p and (window == 0 or p - t < window or t < sink_tokens)
+//
+// The kernels hold scores in the log2 domain (x * log2 e), so the cap and the slopes come multiplied by log2 e.
+#pragma once
+
+#include "common.cuh"
+
+namespace rk {
+
+struct ShapeArgs {
+  float cap = 0.0f;        // cap * log2 e; 0: none
+  float cap_inverse = 0.0f; // 1 / (cap * log2 e)
+  uint32_t window = 0;     // 0: every token up to the row's own
+  uint32_t sinks = 0;      // with a window: tokens that stay visible at the start of the sequence
+  const float *slopes = nullptr; // [query head], device memory; null: none
+};
+
+// Host side: the launch arguments of a shape (null: none). False when a field is out of range.
+inline bool shape_arguments(const rk_score_shape *shape, ShapeArgs &out) {
+  out = ShapeArgs{};
+  if (!shape) return true;
+  if (!(shape->softcap >= 0.0f) || shape->softcap > 1.0e30f || (shape->softcap > 0.0f && shape->softcap < 1.0e-30f)) return false;
+  if (shape->softcap > 0.0f) {
+    out.cap = shape->softcap * 1.4426950408889634f;
+    out.cap_inverse = 1.0f / out.cap;
+  }
+  out.window = shape->window;
+  out.sinks = shape->window ? shape->sink_tokens : 0;
+  out.slopes = shape->slopes;
+  return true;
+}
+
+// cap * tanh(s / cap). tanh(u) = 1 - 2 / (e^2u + 1) loses the small u in the difference from one: its absolute error
+// of about 2^-23 is a relative one of 2^-21 only from |u| = 1/4 on. Below, the odd series u (1 - u^2/3 + 2u^4/15 -
+// 17u^6/315 + 62u^8/2835), whose next term is under 10^-8 there. So the result is good to about 10^-6 of itself
+// whatever the cap is; the hardware's tanh (2^-11) would move a score of 30 by 0.015.
+__device__ __forceinline__ float soft_cap(float s, float cap, float cap_inverse) {
+  const float u = s * cap_inverse, u2 = u * u;
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u * 2.8853900817779268f)); // e^2u
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
+  const float far = fmaf(-2.0f * cap, r, cap);
+  float near = fmaf(u2, 0.021869489f, -0.053968254f);
+  near = fmaf(u2, near, 0.13333333f);
+  near = fmaf(u2, near, -0.33333333f);
+  near = fmaf(u2 * s, near, s);
+  return u2 < 0.0625f ? near : far; // a NaN stays one
+}
+
+// The pages that rows at positions first_position..last_position read, as a list: page(o) for o < count. Pages before
+// `skip` belong to someone else (a shared prefix); of the rest, those with a sink token and those from the first row's
+// window on.
+struct PageList {
+  uint32_t begin, head, gap, count;  // page(o) = begin + o, + gap from o == head on
+  uint32_t window_first;             // first token of the first row's window
+  __device__ __forceinline__ static PageList make(uint32_t first_position, uint32_t last_position, uint32_t skip, const ShapeArgs &shape) {
+    PageList list;
+    const uint32_t pages = last_position / kPageTokens + 1;
+    list.window_first = shape.window && first_position + 1 > shape.window ? first_position + 1 - shape.window : 0;
+    list.begin = min(skip, pages);
+    const uint32_t sinks_end = max(list.begin, rk_pages_for(min(shape.sinks, last_position + 1)));
+    const uint32_t window_begin = max(list.begin, list.window_first / kPageTokens);
+    if (window_begin <= sinks_end) {
+      list.head = list.count = pages - list.begin;
+      list.gap = 0;
+    } else {
+      list.head = sinks_end - list.begin;
+      list.gap = window_begin - sinks_end;
+      list.count = list.head + pages - window_begin;
+    }
+    return list;
+  }
+  __device__ __forceinline__ uint32_t page(uint32_t o) const { return begin + o + (o >= head ? gap : 0); }
+};
+
+// Bit i: the token `base + i` of a page (32-aligned base) is seen by a row at first_position or by one up to `last_position`
+// (`window_first` = first token of the first row's window).
+__device__ __forceinline__ uint32_t seen_tokens(uint32_t base, uint32_t last_position, uint32_t window_first, uint32_t sinks) {
+  auto below = [](uint32_t end) { return end >= 32 ? 0xffffffffu : (1u << end) - 1u; };
+  const uint32_t present = last_position < base ? 0u : below(last_position - base + 1);
+  const uint32_t old = window_first <= base ? 0u : below(window_first - base);
+  const uint32_t sink = sinks <= base ? 0u : below(sinks - base);
+  return present & (~old | sink);
+}
+
+} // namespace rk

@@ -46,6 +46,29 @@ class DecodePlan(C.Structure):
                 ("partials_bytes", C.c_uint64), ("statistics_bytes", C.c_uint64), ("descriptor_bytes", C.c_uint64)]
 
 
+class ScoreShape(C.Structure):
+    """rk_score_shape (include/richkv_abi.h)."""
+    _fields_ = [("softcap", C.c_float), ("window", C.c_uint32), ("sink_tokens", C.c_uint32), ("reserved", C.c_uint32),
+                ("slopes", C.c_void_p)]
+
+
+class StepPool(C.Structure):
+    """rk_step_pool (include/richkv_abi.h)."""
+    _fields_ = [("base", C.c_uint64), ("extent_stride", C.c_uint64), ("extent_pages", C.c_uint32), ("page_count", C.c_uint32)]
+
+
+class SharedPlan(C.Structure):
+    """rk_shared_plan (include/richkv.h)."""
+    _fields_ = [("decode", DecodePlan), ("prefix_ctas", C.c_uint32), ("reserved", C.c_uint32),
+                ("prefix_partials_bytes", C.c_uint64), ("prefix_statistics_bytes", C.c_uint64), ("prefix_descriptor_bytes", C.c_uint64)]
+
+
+class SharedBuffers(C.Structure):
+    """rk_shared_buffers (include/richkv.h)."""
+    _fields_ = [("partials", C.c_void_p), ("statistics", C.c_void_p), ("descriptors", C.c_void_p),
+                ("prefix_partials", C.c_void_p), ("prefix_statistics", C.c_void_p), ("prefix_descriptors", C.c_void_p)]
+
+
 class VerifyBuffers(C.Structure):
     """rk_verify_buffers (include/richkv_host.h)."""
     _fields_ = [("chunk_keys", C.c_void_p), ("chunk_values", C.c_void_p), ("queries", C.c_void_p), ("output", C.c_void_p),
@@ -68,6 +91,8 @@ SIGNATURES = {
     "rk_store_chunk": (i32, [u32, u32, u32, vp, vp, vp, C.POINTER(ChunkParams), vp]),
     "rk_attention_verify_split": (i32, [u32, u32, u32, u32, u32, u32, u32, vp, vp, vp, vp, vp, vp, KvLayer, vp]),
     "rk_attention_verify_split_tc": (i32, [vp, u32, u32, u32, u32, u32, u32, u32, vp, vp, vp, vp, vp, vp, KvLayer, vp, vp]),
+    "rk_attention_verify_split_shaped": (i32, [vp, u32, u32, u32, u32, u32, u32, u32, vp, vp, vp, vp, vp, KvLayer, C.POINTER(ScoreShape), vp, vp]),
+    "rk_attention_prefill_split_shaped": (i32, [vp, u32, u32, u32, u32, vp, vp, vp, vp, C.POINTER(PrefillParams), C.POINTER(ScoreShape), vp, vp]),
     "rk_attention_verify_probe_timeout": (i32, [vp, u32, u32, u32, u32, u32, u32, u32, vp, vp, vp, vp, vp, KvLayer, vp, u32, u32, vp]),
     "rk_attention_verify_reduce": (i32, [u32, u32, u32, u32, u32, vp, vp, vp, vp, vp, vp]),
     "rk_qkv_prepare": (i32, [u32, u32, u32, u32, u32, vp, vp, vp, i32, vp, vp, C.c_float, vp, vp, vp, vp]),
@@ -87,6 +112,11 @@ SIGNATURES = {
     "rk_window_create": (vp, [u64, u64]),
     "rk_window_destroy": (None, [vp]),
     "rk_attention_decode": (i32, [vp, C.POINTER(DecodePlan), u32, vp, vp, vp, vp, vp, vp, vp, vp, KvLayer, vp]),
+    "rk_attention_decode_shaped": (i32, [vp, C.POINTER(DecodePlan), u32, vp, vp, vp, vp, vp, vp, vp, vp, KvLayer, C.POINTER(ScoreShape), vp]),
+    "rk_shared_plan_make": (i32, [u32, u32, u32, u32, u32, u32, C.POINTER(SharedPlan)]),
+    "rk_attention_decode_shared": (i32, [vp, C.POINTER(SharedPlan), u32, vp, vp, vp, C.POINTER(SharedBuffers), vp, vp, KvLayer, vp, vp, C.POINTER(ScoreShape), vp]),
+    "rk_step_tables": (i32, [C.POINTER(StepPool), u32, u32, u32, u32, C.c_float, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "rk_prefix_groups": (i32, [u32, vp, vp, u32, u32, vp, vp, vp]),
     "rk_attention_decode_shard": (i32, [vp, C.POINTER(DecodePlan), u32, vp, vp, vp, vp, vp, vp, vp, KvLayer, vp]),
     "rk_attention_merge_shards": (i32, [u32, u32, u32, u32, u32, vp, vp, vp, vp]),
     "rk_exchange_create": (vp, [u32, u32, u32, vp]),
@@ -118,6 +148,7 @@ SIGNATURES = {
     "rk_storage_is_allocated": (i32, [vp, u32]),
     "rk_storage_window": (None, [vp, C.POINTER(u64), C.POINTER(u64)]),
     "rk_storage_layers": (u32, [vp, C.POINTER(KvLayer), u32]),
+    "rk_storage_step_pool": (None, [vp, C.POINTER(StepPool)]),
     "rk_storage_entry": (u64, [vp, u32]),
     "rk_storage_read_extent": (i32, [vp, u32, u64, vp, u64]),
     "rk_storage_write_extent": (i32, [vp, u32, u64, vp, u64]),

@@ -18,7 +18,7 @@ import numpy as np
 import torch
 
 from . import lib
-from .abi import CHUNK_PARAMS, VERIFY_PARAMS, Layout
+from .abi import CHUNK_PARAMS, TREE_NODES, VERIFY_PARAMS, Layout
 
 
 def _stream(stream) -> int:
@@ -61,6 +61,25 @@ def attention_verify_split(layout: Layout, query_heads: int, lanes: int, row_cap
     lib.check(status, "rk_attention_verify_split")
 
 
+class ScoreShape:
+    """What a score goes through before the softmax (rk_score_shape): `softcap` * tanh(score / softcap), minus slope *
+    distance per query head, seen only inside a sliding `window` (the first `sink_tokens` stay visible beside it)."""
+
+    def __init__(self, softcap: float = 0.0, window: int = 0, sink_tokens: int = 0, slopes=None):
+        if not 0.0 <= softcap < float("inf"):
+            raise ValueError("ScoreShape: softcap must be finite and not negative")
+        if not 0 <= window < 2 ** 32 or not 0 <= sink_tokens < 2 ** 32:
+            raise ValueError("ScoreShape: window and sink_tokens are counts of tokens")
+        if slopes is not None and (slopes.dtype != torch.float32 or not slopes.is_cuda or not slopes.is_contiguous() or slopes.dim() != 1):
+            raise ValueError("ScoreShape: slopes is a contiguous fp32 device vector, one per query head")
+        self.softcap, self.window, self.sink_tokens, self.slopes = softcap, window, sink_tokens, slopes
+
+    def block(self, query_heads: int) -> lib.ScoreShape:
+        if self.slopes is not None and self.slopes.numel() != query_heads:
+            raise ValueError(f"ScoreShape: {self.slopes.numel()} slopes for {query_heads} query heads")
+        return lib.ScoreShape(self.softcap, self.window, self.sink_tokens, 0, self.slopes.data_ptr() if self.slopes is not None else None)
+
+
 class VerifyWindowAttention:
     """8/16-row int4 verify windows on the tcgen05 split kernel (rk_attention_verify_split_tc).
 
@@ -84,7 +103,17 @@ class VerifyWindowAttention:
         self.close()
 
     def split(self, lanes: int, row_capacity: int, grid_splits: int, queries, partials, statistics, table_pointers,
-              row_masks, params, layer: lib.KvLayer, stream=None) -> None:
+              row_masks, params, layer: lib.KvLayer, stream=None, shape: ScoreShape | None = None) -> None:
+        if shape is not None:  # chain windows of 8 or 16 rows
+            if row_masks is not None:
+                raise ValueError("a score shape goes with chain windows, not with tree masks")
+            status = self._lib.rk_attention_verify_split_shaped(
+                self._window, self.layout.format, self.layout.kv_heads, self.query_heads, self.layout.head_dimension,
+                lanes, row_capacity, grid_splits, queries.data_ptr(), partials.data_ptr(), statistics.data_ptr(),
+                table_pointers.data_ptr(), params.data_ptr(), layer, C.byref(shape.block(self.query_heads)),
+                self.status_word.data_ptr(), _stream(stream))
+            lib.check(status, "rk_attention_verify_split_shaped")
+            return
         status = self._lib.rk_attention_verify_split_tc(
             self._window, self.layout.format, self.layout.kv_heads, self.query_heads, self.layout.head_dimension,
             lanes, row_capacity, grid_splits, queries.data_ptr(), partials.data_ptr(), statistics.data_ptr(),
@@ -92,8 +121,16 @@ class VerifyWindowAttention:
             layer, self.status_word.data_ptr(), _stream(stream))
         lib.check(status, "rk_attention_verify_split_tc")
 
-    def prefill_split(self, queries, partials, statistics, table, params: lib.PrefillParams, stream=None) -> None:
+    def prefill_split(self, queries, partials, statistics, table, params: lib.PrefillParams, stream=None,
+                      shape: ScoreShape | None = None) -> None:
         """The 8-row tiles of a prefill chunk (rk_attention_prefill_split_tc); merge with attention_prefill_reduce."""
+        if shape is not None:
+            status = self._lib.rk_attention_prefill_split_shaped(
+                self._window, self.layout.format, self.layout.kv_heads, self.query_heads, self.layout.head_dimension,
+                queries.data_ptr(), partials.data_ptr(), statistics.data_ptr(), table.data_ptr(), C.byref(params),
+                C.byref(shape.block(self.query_heads)), self.status_word.data_ptr(), _stream(stream))
+            lib.check(status, "rk_attention_prefill_split_shaped")
+            return
         status = self._lib.rk_attention_prefill_split_tc(
             self._window, self.layout.format, self.layout.kv_heads, self.query_heads, self.layout.head_dimension,
             queries.data_ptr(), partials.data_ptr(), statistics.data_ptr(), table.data_ptr(), C.byref(params),
@@ -244,7 +281,16 @@ class DecodeAttention:
         except Exception:
             pass
 
-    def run(self, queries, output, table_pointers, params, layer: lib.KvLayer, output_f32=None, stream=None):
+    def run(self, queries, output, table_pointers, params, layer: lib.KvLayer, output_f32=None, stream=None,
+            shape: ScoreShape | None = None):
+        if shape is not None:
+            status = self._lib.rk_attention_decode_shaped(
+                self._window, C.byref(self.plan), self.layout.format, queries.data_ptr(), output.data_ptr(),
+                output_f32.data_ptr() if output_f32 is not None else None, self.partials.data_ptr(),
+                self.statistics.data_ptr(), self.descriptors.data_ptr(), table_pointers.data_ptr(), params.data_ptr(),
+                layer, C.byref(shape.block(self.query_heads)), _stream(stream))
+            lib.check(status, "rk_attention_decode_shaped")
+            return
         status = self._lib.rk_attention_decode(
             self._window, C.byref(self.plan), self.layout.format, queries.data_ptr(), output.data_ptr(),
             output_f32.data_ptr() if output_f32 is not None else None, self.partials.data_ptr(),
@@ -256,3 +302,125 @@ class DecodeAttention:
         """Raises if a bounded device wait ran out during the steps launched so far."""
         lib.check(self._lib.rk_attention_decode_status(C.byref(self.plan), self.descriptors.data_ptr(), _stream(stream)),
                   "rk_attention_decode_status")
+
+
+class StepTables:
+    """A step's page tables, parameter blocks and row slots, built on the GPU from request lengths (rk_step_tables).
+
+    `window`, `extent_stride`, `extent_pages` and `page_count` say where page ids lie (for_storage takes them from a
+    PageStorage); build() fills `entries`, `chunk_params`, `verify_params`, `row_offsets` and `row_slots` in stream order, and the
+    stores and attention kernels take `table_pointers` and the parameter blocks as they are."""
+
+    def __init__(self, lanes: int, table_pages: int, window: tuple[int, int], extent_stride: int, extent_pages: int,
+                 page_count: int, row_capacity: int = 1, split_count: int = 1, score_scale: float = 0.0):
+        if lanes < 1 or table_pages < 1 or not 1 <= row_capacity <= TREE_NODES:
+            raise ValueError("StepTables: lanes, table pages and a row capacity of at most 16")
+        self._lib = lib.load()
+        self.lanes, self.table_pages, self.row_capacity = lanes, table_pages, row_capacity
+        self.split_count, self.score_scale = split_count, score_scale
+        self._pool = lib.StepPool(window[0], extent_stride, extent_pages, page_count)
+        self.entries = torch.zeros((lanes, table_pages), dtype=torch.int64, device="cuda")
+        self.table_pointers = self.entries.data_ptr() + 8 * table_pages * torch.arange(lanes, dtype=torch.int64, device="cuda")
+        self.chunk_params = torch.zeros((lanes, CHUNK_PARAMS.itemsize), dtype=torch.uint8, device="cuda")
+        self.verify_params = torch.zeros((lanes, VERIFY_PARAMS.itemsize), dtype=torch.uint8, device="cuda")
+        self.row_offsets = torch.zeros(lanes + 1, dtype=torch.int32, device="cuda")
+        self.row_slots = torch.zeros(lanes * row_capacity, dtype=torch.int64, device="cuda")
+        self.status_word = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    @classmethod
+    def for_storage(cls, storage, lanes: int, table_pages: int, row_capacity: int = 1, split_count: int = 1,
+                    score_scale: float = 0.0) -> "StepTables":
+        pool = storage.step_pool()
+        return cls(lanes, table_pages, storage.window(), pool.extent_stride, pool.extent_pages, pool.page_count, row_capacity, split_count,
+                   score_scale)
+
+    def build(self, page_ids, page_offsets, committed, rows, known_pages=None, stream=None) -> None:
+        """Per lane l: page ids page_ids[page_offsets[l] : page_offsets[l + 1]], committed tokens, new rows (0: idle);
+        entries before known_pages[l] stay as they are. All int32 device vectors."""
+        for name, vector, size in (("page_ids", page_ids, None), ("page_offsets", page_offsets, self.lanes + 1),
+                                   ("committed", committed, self.lanes), ("rows", rows, self.lanes), ("known_pages", known_pages, self.lanes)):
+            if vector is None and name == "known_pages":
+                continue
+            if vector.dtype != torch.int32 or not vector.is_contiguous() or vector.device != self.entries.device or \
+                    (size is not None and vector.numel() != size):
+                raise ValueError(f"StepTables.build: {name} is a contiguous int32 vector on the tables' device" +
+                                 (f" of {size}" if size else ""))
+        status = self._lib.rk_step_tables(
+            C.byref(self._pool), self.lanes, self.table_pages, self.row_capacity, self.split_count, self.score_scale,
+            page_ids.data_ptr(), page_offsets.data_ptr(), committed.data_ptr(), rows.data_ptr(),
+            known_pages.data_ptr() if known_pages is not None else None, self.entries.data_ptr(), self.chunk_params.data_ptr(),
+            self.verify_params.data_ptr(), self.row_offsets.data_ptr(), self.row_slots.data_ptr(), self.status_word.data_ptr(),
+            _stream(stream))
+        lib.check(status, "rk_step_tables")
+
+    def check(self) -> None:
+        """Synchronises, raises if a lane was refused since the last check, and clears the word."""
+        if int(self.status_word.item()):
+            self.status_word.zero_()
+            raise lib.RichKvError(lib.INVALID, "rk_step_tables: a lane asks for rows, tokens or pages it cannot have")
+
+
+def prefix_groups(lanes: int, table_pointers, params, lane_groups, group_pages, minimum_lanes: int = 2, minimum_pages: int = 1,
+                  stream=None) -> None:
+    """Which lanes share how long a prefix, from their page tables (rk_prefix_groups): lane_groups[l] = the lowest lane
+    of l's group or -1, group_pages[that lane] = the pages they share. Both int32 device vectors of `lanes`."""
+    for name, vector in (("lane_groups", lane_groups), ("group_pages", group_pages)):
+        if vector.dtype != torch.int32 or not vector.is_contiguous() or vector.numel() != lanes:
+            raise ValueError(f"prefix_groups: {name} is a contiguous int32 vector of {lanes}")
+    status = lib.load().rk_prefix_groups(lanes, table_pointers.data_ptr(), params.data_ptr(), minimum_lanes, minimum_pages,
+                                         lane_groups.data_ptr(), group_pages.data_ptr(), _stream(stream))
+    lib.check(status, "rk_prefix_groups")
+
+
+class SharedPrefixDecode:
+    """Decode attention for a batch in which groups of lanes share the first pages of their tables
+    (rk_attention_decode_shared): a group's prefix is read once for all of its lanes. Holds the window's tensor maps and
+    the step's scratch; lane_groups and group_pages are prefix_groups' output (or a caller's own in that form)."""
+
+    def __init__(self, layout: Layout, query_heads: int, lanes: int, window: tuple[int, int], ctas: int = 0):
+        self._lib = lib.load()
+        self.layout, self.query_heads, self.lanes = layout, query_heads, lanes
+        self.plan = lib.SharedPlan()
+        self._window = None
+        lib.check(self._lib.rk_shared_plan_make(layout.format, layout.kv_heads, query_heads, layout.head_dimension, lanes, ctas,
+                                                C.byref(self.plan)), "rk_shared_plan_make")
+        self._window = self._lib.rk_window_create(window[0], window[1])
+        if not self._window:
+            raise lib.RichKvError(lib.INVALID, "rk_window_create")
+        decode = self.plan.decode
+        self.partials = torch.empty(decode.partials_bytes // 4, dtype=torch.float32, device="cuda")
+        self.statistics = torch.empty(decode.statistics_bytes // 4, dtype=torch.float32, device="cuda")
+        self.descriptors = torch.zeros(decode.descriptor_bytes // 4, dtype=torch.int32, device="cuda")
+        self.prefix_partials = torch.empty(self.plan.prefix_partials_bytes // 4, dtype=torch.float32, device="cuda")
+        self.prefix_statistics = torch.empty(self.plan.prefix_statistics_bytes // 4, dtype=torch.float32, device="cuda")
+        self.prefix_descriptors = torch.zeros(self.plan.prefix_descriptor_bytes // 4, dtype=torch.int32, device="cuda")
+        self._buffers = lib.SharedBuffers(*(t.data_ptr() for t in (self.partials, self.statistics, self.descriptors, self.prefix_partials,
+                                                                   self.prefix_statistics, self.prefix_descriptors)))
+
+    def close(self):
+        if self._window:
+            self._lib.rk_window_destroy(self._window)
+            self._window = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def run(self, queries, output, table_pointers, params, layer: lib.KvLayer, lane_groups, group_pages, output_f32=None,
+            stream=None, shape: ScoreShape | None = None):
+        for name, vector in (("lane_groups", lane_groups), ("group_pages", group_pages)):
+            if vector.dtype != torch.int32 or not vector.is_contiguous() or vector.numel() != self.lanes:
+                raise ValueError(f"SharedPrefixDecode.run: {name} is a contiguous int32 vector of {self.lanes}")
+        block = C.byref(shape.block(self.query_heads)) if shape is not None else None
+        status = self._lib.rk_attention_decode_shared(
+            self._window, C.byref(self.plan), self.layout.format, queries.data_ptr(), output.data_ptr(),
+            output_f32.data_ptr() if output_f32 is not None else None, C.byref(self._buffers), table_pointers.data_ptr(),
+            params.data_ptr(), layer, lane_groups.data_ptr(), group_pages.data_ptr(), block, _stream(stream))
+        lib.check(status, "rk_attention_decode_shared")
+
+    def status(self, stream=None) -> None:
+        """Raises if a bounded device wait ran out during the steps launched so far."""
+        lib.check(self._lib.rk_attention_decode_status(C.byref(self.plan.decode), self.descriptors.data_ptr(), _stream(stream)),
+                  "rk_attention_decode_shared")

@@ -82,6 +82,12 @@ class PageStorage:
         self._lib.rk_storage_window(self._handle, C.byref(base), C.byref(size))
         return base.value, size.value
 
+    def step_pool(self) -> lib.StepPool:
+        """Where page ids lie, for tables built on the GPU (ops.StepTables)."""
+        pool = lib.StepPool()
+        self._lib.rk_storage_step_pool(self._handle, C.byref(pool))
+        return pool
+
     def layers(self) -> list[lib.KvLayer]:
         count = self.layout.attention_layers
         out = (lib.KvLayer * count)()

@@ -1,0 +1,229 @@
+"""GPU: score shapes (tanh cap, sliding window with sinks, distance bias) on the streaming decode kernels, the verify
+windows and the prefill tiles, against attention in 64 bits from the pages' bytes."""
+import numpy as np
+import pytest
+import torch
+
+from gpuhelp import dev
+from richengine_b200 import lib, ops
+from richengine_b200.abi import BF16, FP8E4M3, INT4, INT8
+from servingcase import (DIM, FORMATS, GROUP, HEADS, PAGE, SLOPES, Batch, check_rows, host16, make_queries, shape_of, shuffled_pages)
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = {
+    "cap": (3.0, 0, 0, None),
+    "wide cap": (1.0e5, 0, 0, None),
+    "window 1": (0.0, 1, 0, None),
+    "window 32": (0.0, 32, 0, None),
+    "window 33, sinks": (0.0, 33, 5, None),
+    "window 200, sinks over pages": (0.0, 200, 70, None),
+    "window past everything": (0.0, 2 ** 32 - 1, 2 ** 32 - 1, None),
+    "bias": (0.0, 0, 0, SLOPES),
+    "all": (5.0, 100, 33, SLOPES),
+}
+CONTEXTS = [0, 31, 32, 700, 64, 1055]
+
+
+def decode(batch, committed, queries, shape, ctas=0, fill=float("nan"), params=None):
+    runner = ops.DecodeAttention(batch.layout, 24, batch.lanes, batch.storage.window(), ctas)
+    runner.partials.fill_(fill)
+    runner.statistics.fill_(fill)
+    q = dev(queries)
+    out = torch.zeros(q.shape, dtype=torch.bfloat16, device="cuda")
+    out32 = torch.zeros(q.shape, dtype=torch.float32, device="cuda")
+    runner.run(q, out, batch.pointers, params if params is not None else batch.params(committed), batch.layer, output_f32=out32, shape=shape)
+    runner.status()
+    runner.close()
+    return host16(out), out32.cpu().numpy()
+
+
+def prepared(fmt, contexts, rows=1, seed=5):
+    rng = np.random.default_rng(seed)
+    batch = Batch(fmt, shuffled_pages(rng, [-(-(c + rows) // PAGE) for c in contexts]), seed)
+    return batch, make_queries(rng, len(contexts), HEADS, 32, GROUP, DIM)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("name", SHAPES)
+def test_decode(fmt, name):
+    batch, q = prepared(fmt, CONTEXTS)
+    shape = SHAPES[name]
+    for ctas in (0, 3):
+        got16, got32 = decode(batch, CONTEXTS, q, shape_of(shape), ctas)
+        for lane, context in enumerate(CONTEXTS):
+            want, bound = batch.attend(lane, context, q[lane, :, 0], shape)
+            check_rows(got32[lane, :, 0], got16[lane, :, 0], want, bound, f"{name}, lane {lane}, ctas {ctas}")
+        assert not got16[:, :, 1:].any()
+    batch.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_an_empty_shape_changes_nothing(fmt):
+    batch, q = prepared(fmt, CONTEXTS)
+    plain16, plain32 = decode(batch, CONTEXTS, q, None)
+    got16, got32 = decode(batch, CONTEXTS, q, ops.ScoreShape())
+    assert np.array_equal(plain16, got16) and np.array_equal(plain32, got32)
+    batch.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_unseen_tokens_may_hold_anything(fmt):
+    """Everything outside the window and the sinks, on seen pages too, and everything behind the last token is 0xFF:
+    NaN where the format has one, NaN scales elsewhere."""
+    context, window, sinks = 500, 77, 37
+    batch, q = prepared(fmt, [context])
+    seen = [t for t in range(len(batch.pages[0]) * PAGE) if t <= context and (t > context - window or t < sinks)]
+    kept = {}
+    keys_shape = {INT4: (HEADS, PAGE, DIM // 2), BF16: (HEADS, PAGE, DIM * 2)}.get(fmt, (HEADS, PAGE, DIM))
+    for t in range(len(batch.pages[0]) * PAGE):
+        if t in seen:
+            continue
+        page, at = batch.pages[0][t // PAGE], t % PAGE
+        keys, key_scales, values, value_scales = (batch.host.tensor_view(page, 0, i) for i in range(4))
+        keys.reshape(keys_shape)[:, at] = 0xff
+        if fmt == INT4:
+            values.reshape(keys_shape)[:, at] = 0xff
+        else:
+            values.reshape(HEADS, DIM, PAGE, -1)[:, :, at] = 0xff
+        if fmt != BF16:
+            key_scales.view(np.uint32).reshape(HEADS, PAGE)[:, at] = 0xffffffff
+            value_scales.view(np.uint32).reshape(HEADS, PAGE)[:, at] = 0xffffffff
+    batch.upload()
+    shape = (20.0, window, sinks, SLOPES)
+    want, bound = batch.attend(0, context, q[0, :, 0], shape)
+    got16, got32 = decode(batch, [context], q, shape_of(shape))
+    check_rows(got32[0, :, 0], got16[0, :, 0], want, bound, "decode")
+    # the same row as the only live one of a verify window and of a prefill chunk
+    got16, got32 = verify(batch, [context], 1, 8, q, shape_of(shape), splits=3)
+    check_rows(got32[0, :, 0], got16[0, :, 0], want, bound, "verify")
+    got16, got32 = prefill(batch, context, 1, q[0], shape_of(shape), splits=2)
+    check_rows(got32[:, 0], got16[:, 0], want, bound, "prefill")
+    batch.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_the_last_position_of_the_longest_context(fmt):
+    """A table of 8 192 entries over a few pages: offsets past 32 bits of scores and of distance, windows at the far end."""
+    rng = np.random.default_rng(2)
+    committed = 262143
+    batch = Batch(fmt, [list(rng.integers(0, 60, 8192))], 2)
+    q = make_queries(rng, 1, HEADS, 32, GROUP, DIM)
+    for shape in ((0.0, 129, 3, SLOPES), (7.0, 4001, 0, None)):
+        want, bound = batch.attend(0, committed, q[0, :, 0], shape)
+        got16, got32 = decode(batch, [committed], q, shape_of(shape))
+        check_rows(got32[0, :, 0], got16[0, :, 0], want, bound, "decode")
+    batch.close()
+
+
+@pytest.mark.parametrize("fmt", [INT4, BF16])
+def test_idle_and_refused_lanes_are_left_as_they_are(fmt):
+    batch, q = prepared(fmt, [100, 200, 300])
+    params = batch.params([100, 200, 300], rows=[1, 0, 1])
+    runner_shape = shape_of((0.0, 50, 4, None))
+    got16, got32 = decode(batch, [100, 200, 300], q, runner_shape, params=params)
+    assert not got16[1].any() and not got32[1].any()
+    for lane, context in ((0, 100), (2, 300)):
+        want, bound = batch.attend(lane, context, q[lane, :, 0], (0.0, 50, 4, None))
+        check_rows(got32[lane, :, 0], got16[lane, :, 0], want, bound, f"lane {lane}")
+    batch.close()
+
+
+@pytest.mark.parametrize("fmt", [INT4, FP8E4M3])
+def test_many_lanes_and_large_scores(fmt):
+    """More lanes than CTAs; scores far past the cap (the tanh saturates) and a scale of the caller's own."""
+    rng = np.random.default_rng(9)
+    contexts = [int(c) for c in rng.integers(0, 90, 200)]
+    batch, q = prepared(fmt, contexts, seed=9)
+    runner = batch.params(contexts, score_scale=0.5)
+    shape = (15.0, 40, 2, SLOPES)
+    got16, got32 = decode(batch, contexts, q, shape_of(shape), params=runner)
+    for lane in range(0, 200, 7):
+        want, bound = batch.attend(lane, contexts[lane], q[lane, :, 0], shape, scale=0.5)
+        check_rows(got32[lane, :, 0], got16[lane, :, 0], want, bound, f"lane {lane}")
+    batch.close()
+
+
+# ---- verify windows -------------------------------------------------------------------------------------------------
+
+def verify(batch, committed, rows, capacity, queries, shape, splits):
+    params = batch.params(committed, rows, capacity, splits)
+    slots = batch.lanes * HEADS * splits * capacity * GROUP
+    partials = torch.full((slots * DIM,), float("nan"), device="cuda")
+    statistics = torch.full((slots * 2,), float("nan"), device="cuda")
+    q = dev(queries)
+    out, out32 = torch.zeros(q.shape, dtype=torch.bfloat16, device="cuda"), torch.zeros(q.shape, dtype=torch.float32, device="cuda")
+    runner = ops.VerifyWindowAttention(batch.layout, 24, batch.storage.window())
+    runner.split(batch.lanes, capacity, splits, q, partials, statistics, batch.pointers, None, params, batch.layer, shape=shape)
+    ops.attention_verify_reduce(batch.layout, 24, batch.lanes, capacity, partials, statistics, out, params, output_f32=out32)
+    runner.check()
+    runner.close()
+    return host16(out), out32.cpu().numpy()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("name", SHAPES)
+@pytest.mark.parametrize("rows,capacity,splits", [(8, 8, 1), (11, 16, 3), (16, 16, 9), (1, 8, 4)])
+def test_verify(fmt, name, rows, capacity, splits):
+    contexts = [0, 31, 300, 64]
+    batch, q = prepared(fmt, contexts, rows)
+    shape = SHAPES[name]
+    got16, got32 = verify(batch, contexts, rows, capacity, q, shape_of(shape), splits)
+    for lane, context in enumerate(contexts):
+        for r in sorted({0, rows // 2, rows - 1}):
+            want, bound = batch.attend(lane, context + r, q[lane, :, r], shape)
+            check_rows(got32[lane, :, r], got16[lane, :, r], want, bound, f"{name}, lane {lane}, row {r}")
+    assert not got16[:, :, rows:].any()
+    batch.close()
+
+
+# ---- prefill tiles --------------------------------------------------------------------------------------------------
+
+def prefill(batch, committed, rows, queries, shape, splits):
+    """queries [head][stride][group][dim] bf16 bits."""
+    stride = queries.shape[1]
+    params = lib.PrefillParams(committed, rows, stride, len(batch.pages[0]), batch.layer, splits, 0.0)
+    tiles = -(-rows // 8)
+    slots = tiles * HEADS * splits * 8 * GROUP
+    partials = torch.full((slots * DIM,), float("nan"), device="cuda")
+    statistics = torch.full((slots * 2,), float("nan"), device="cuda")
+    q = dev(queries)
+    out, out32 = torch.zeros(q.shape, dtype=torch.bfloat16, device="cuda"), torch.zeros(q.shape, dtype=torch.float32, device="cuda")
+    runner = ops.VerifyWindowAttention(batch.layout, 24, batch.storage.window())
+    runner.prefill_split(q, partials, statistics, batch.tables[0], params, shape=shape)
+    ops.attention_prefill_reduce(batch.layout, 24, partials, statistics, out, params, output_f32=out32)
+    runner.check()
+    runner.close()
+    return host16(out), out32.cpu().numpy()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("name", SHAPES)
+@pytest.mark.parametrize("committed,rows,splits", [(0, 1, 4), (0, 33, 1), (170, 21, 3), (300, 100, 1), (77, 8, 5)])
+def test_prefill(fmt, name, committed, rows, splits):
+    batch, _ = prepared(fmt, [committed], rows)
+    q = make_queries(np.random.default_rng(rows), HEADS, -(-rows // 32) * 32, GROUP, DIM)
+    shape = SHAPES[name]
+    got16, got32 = prefill(batch, committed, rows, q, shape_of(shape), splits)
+    for r in sorted({0, 7, 8, rows // 2, rows - 1} & set(range(rows))):
+        want, bound = batch.attend(0, committed + r, q[:, r], shape)
+        check_rows(got32[:, r], got16[:, r], want, bound, f"{name}, row {r}")
+    batch.close()
+
+
+def test_refusals():
+    batch, q = prepared(INT4, [40], 8)
+    shape = ops.ScoreShape(softcap=10.0)
+    runner = ops.VerifyWindowAttention(batch.layout, 24, batch.storage.window())
+    scratch, masks = torch.zeros(8, device="cuda"), torch.zeros(16, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="chain windows"):
+        runner.split(1, 8, 1, scratch, scratch, scratch, batch.pointers, masks, scratch, batch.layer, shape=shape)
+    with pytest.raises(lib.RichKvError, match="rk_attention_decode_shaped"):
+        runner.split(1, 1, 1, scratch, scratch, scratch, batch.pointers, None, scratch, batch.layer, shape=shape)
+    with pytest.raises(ValueError, match="24 query heads"):
+        decode(batch, [40], q, ops.ScoreShape(slopes=torch.ones(23, device="cuda")))
+    for slopes in (torch.ones(24), torch.ones(24, dtype=torch.float64, device="cuda"), torch.ones(24, 2, device="cuda")[:, 0]):
+        with pytest.raises(ValueError, match="slopes"):
+            ops.ScoreShape(slopes=slopes)
+    runner.close()
+    batch.close()

@@ -1,0 +1,256 @@
+"""GPU: decode attention over shared prefixes against attention in 64 bits from the pages' bytes, and the whole step:
+tables from request lengths, groups from the tables, append, attention, as eager calls and as a replayed graph."""
+import numpy as np
+import pytest
+import torch
+
+from gpuhelp import dev
+from richengine_b200 import lib, ops
+from richengine_b200.abi import BF16, FP8E4M3, INT4, INT8
+from servingcase import DIM, FORMATS, GROUP, HEADS, PAGE, SLOPES, Batch, check_rows, host16, make_queries, shape_of
+
+pytestmark = pytest.mark.gpu
+
+
+class Shared:
+    """`groups`: (prefix pages, members) each; `loose` lanes share nothing. Lanes of all groups are mixed."""
+
+    def __init__(self, fmt, groups, loose=0, suffix=70, seed=4, members_first=False):
+        rng = np.random.default_rng(seed)
+        member = [g for g, (_, n) in enumerate(groups) for _ in range(n)] + [-1] * loose
+        if not members_first:
+            rng.shuffle(member)
+        lanes = len(member)
+        tokens = rng.integers(1, suffix + 1, lanes)  # past the prefix, this step's own among them
+        own = [-(-int(t) // PAGE) for t in tokens]
+        ids = iter(rng.permutation(sum(p for p, _ in groups) + sum(own)))
+        prefixes = [[next(ids) for _ in range(p)] for p, _ in groups]
+        pages = [(prefixes[g] if g >= 0 else []) + [next(ids) for _ in range(own[l])] for l, g in enumerate(member)]
+        self.committed = [(len(prefixes[g]) * PAGE if g >= 0 else 0) + int(tokens[l]) - 1 for l, g in enumerate(member)]
+        self.member, self.lanes = member, lanes
+        self.batch = Batch(fmt, pages, seed)
+        self.queries = make_queries(rng, lanes, HEADS, 32, GROUP, DIM)
+        names = list(rng.permutation(lanes)[:len(groups)])  # any number below `lanes` names a group
+        self.lane_groups = dev(np.array([names[g] if g >= 0 else -1 for g in member], np.int32))
+        group_pages = np.zeros(lanes, np.int32)
+        for g, (p, _) in enumerate(groups):
+            group_pages[names[g]] = p
+        self.group_pages = dev(group_pages)
+
+    def run(self, shape=None, ctas=0, params=None, runner=None, lane_groups=None):
+        b = self.batch
+        own = runner is None
+        if own:
+            runner = ops.SharedPrefixDecode(b.layout, 24, self.lanes, b.storage.window(), ctas)
+            for scratch in (runner.partials, runner.statistics, runner.prefix_partials, runner.prefix_statistics):
+                scratch.fill_(float("nan"))
+            runner.prefix_descriptors.fill_(0x7f7f7f7f)
+        q = dev(self.queries)
+        out = torch.zeros(q.shape, dtype=torch.bfloat16, device="cuda")
+        out32 = torch.zeros(q.shape, dtype=torch.float32, device="cuda")
+        runner.run(q, out, b.pointers, params if params is not None else b.params(self.committed), b.layer,
+                   lane_groups if lane_groups is not None else self.lane_groups, self.group_pages, output_f32=out32,
+                   shape=shape_of(shape) if shape else None)
+        runner.status()
+        if own:
+            runner.close()
+        return host16(out), out32.cpu().numpy()
+
+    def check(self, got16, got32, shape=None, lanes=None, scale=1.0 / 16.0):
+        for lane in lanes if lanes is not None else range(self.lanes):
+            want, bound = self.batch.attend(lane, self.committed[lane], self.queries[lane, :, 0], shape, scale)
+            # two partials meet in the merge: their weights' exponentials and the sum add a few roundings of 2^-23
+            check_rows(got32[lane, :, 0], got16[lane, :, 0], want, bound + 2.0 ** -20 * np.abs(want).max(), f"lane {lane}")
+        assert not got16[:, :, 1:].any()
+
+
+GROUPS = {
+    "one page, two lanes": ([(1, 2)], 0),
+    "one lane alone": ([(3, 1)], 2),
+    "a tile and its neighbours": ([(2, 21), (3, 22), (1, 43)], 0),
+    "odd pages": ([(7, 5), (1, 3), (10, 4)], 3),
+    "a long prefix": ([(40, 6)], 1),
+    "nobody shares": ([], 4),
+}
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("name", GROUPS)
+def test_against_64_bits(fmt, name):
+    groups, loose = GROUPS[name]
+    s = Shared(fmt, groups, loose)
+    pick = sorted(set(range(0, s.lanes, max(1, s.lanes // 8))) | {s.lanes - 1})
+    for ctas in (0, 5):  # five CTAs: more tiles than CTAs, each CTA takes several
+        s.check(*s.run(ctas=ctas), lanes=pick)
+    s.batch.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("shape", [(4.0, 0, 0, None), (0.0, 0, 0, SLOPES), (0.0, 60, 3, None), (6.0, 150, 40, SLOPES), (0.0, 1, 0, None)])
+def test_with_a_score_shape(fmt, shape):
+    s = Shared(fmt, [(5, 6), (3, 2)], 2)
+    s.check(*s.run(shape), shape)
+    s.batch.close()
+
+
+@pytest.mark.parametrize("fmt", [INT4, BF16])
+def test_equals_the_plain_decode(fmt):
+    """The same batch without its groups is rk_attention_decode's business: same rows up to the bound, and bit for bit
+    when no lane belongs to a group."""
+    s = Shared(fmt, [(9, 30)], 5)
+    b = s.batch
+    alone = dev(np.full(s.lanes, -1, np.int32))
+    none16, none32 = s.run(lane_groups=alone)
+    shared16, shared32 = s.run()
+    s.check(none16, none32, lanes=range(0, s.lanes, 5))
+    s.check(shared16, shared32, lanes=range(0, s.lanes, 5))
+    plain = ops.DecodeAttention(b.layout, 24, s.lanes, b.storage.window())
+    q = dev(s.queries)
+    out32 = torch.zeros(q.shape, dtype=torch.float32, device="cuda")
+    plain.run(q, torch.zeros(q.shape, dtype=torch.bfloat16, device="cuda"), b.pointers, b.params(s.committed), b.layer, output_f32=out32)
+    # the merges divide differently (a reciprocal against a division) and group their slots differently: 2^-20 of a row's largest
+    difference = np.abs(out32.cpu().numpy() - none32)
+    assert difference.max() <= 2.0 ** -20 * np.abs(none32).max()
+    plain.close()
+    b.close()
+
+
+def test_repeats_bit_for_bit_and_scratch_is_reused():
+    s = Shared(INT4, [(12, 25), (4, 3)], 2)
+    b = s.batch
+    runner = ops.SharedPrefixDecode(b.layout, 24, s.lanes, b.storage.window())
+    first = s.run(runner=runner)
+    other = s.run((3.0, 0, 0, None), runner=runner)
+    again = s.run(runner=runner)
+    assert np.array_equal(first[0], again[0]) and np.array_equal(first[1], again[1]) and not np.array_equal(first[1], other[1])
+    runner.close()
+    b.close()
+
+
+@pytest.mark.parametrize("fmt", [INT8, FP8E4M3])
+def test_idle_lanes(fmt):
+    """Idle members and idle leaders: the others of their group go on, the idle ones' rows stay as they are."""
+    s = Shared(fmt, [(3, 6), (2, 2)], 2)
+    rows = [1] * s.lanes
+    for g in (0, 1):
+        rows[s.member.index(g)] = 0  # the lowest member of each
+    got16, got32 = s.run(params=s.batch.params(s.committed, rows=rows))
+    idle = [l for l in range(s.lanes) if not rows[l]]
+    assert not got16[idle].any() and not got32[idle].any()
+    s.check(got16, got32, lanes=[l for l in range(s.lanes) if rows[l]])
+    s.batch.close()
+
+
+@pytest.mark.parametrize("fmt", [INT4, BF16])
+def test_a_prefix_that_covers_everything(fmt):
+    """Every committed page shared and the step's own token alone behind it; and a batch whose lanes lie inside the prefix
+    (no lane has anything to stream)."""
+    s = Shared(fmt, [(4, 9)], 0, suffix=1)
+    s.check(*s.run())
+    s.committed = [127 - l for l in range(s.lanes)]  # rows of the prefix itself
+    s.check(*s.run(ctas=3))
+    s.batch.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_many_lanes(fmt):
+    s = Shared(fmt, [(6, 300), (3, 40)], 60, suffix=40)
+    s.check(*s.run(), lanes=range(0, s.lanes, 37))
+    s.batch.close()
+
+
+@pytest.mark.parametrize("fmt", [INT4, FP8E4M3])
+def test_large_queries_and_peaked_rows(fmt):
+    s = Shared(fmt, [(10, 8)], 1)
+    s.queries = (s.queries.astype(np.int32) + (3 << 7)).astype(np.uint16)  # x 8 (three more in the exponent)
+    got16, got32 = s.run()
+    s.check(got16, got32)
+    s.queries = (s.queries.astype(np.int32) + (12 << 7)).astype(np.uint16)  # past fp16's range: a power of two keeps it
+    params = s.batch.params(s.committed, score_scale=2.0 ** -16)
+    got16, got32 = s.run(params=params)
+    s.check(got16, got32, scale=2.0 ** -16)
+    s.batch.close()
+
+
+def test_refusals():
+    s = Shared(INT4, [(1, 2)], 0)
+    b = s.batch
+    with pytest.raises(lib.RichKvError, match="lanes out of range"):
+        ops.SharedPrefixDecode(b.layout, 24, 1025, b.storage.window())
+    with pytest.raises(lib.RichKvError, match="4 KV heads"):
+        ops.SharedPrefixDecode(b.layout, 32, 4, b.storage.window())
+    runner = ops.SharedPrefixDecode(b.layout, 24, 2, b.storage.window())
+    with pytest.raises(ValueError, match="lane_groups"):
+        s.run(runner=runner, lane_groups=dev(np.zeros(3, np.int32)))
+    runner.close()
+    b.close()
+
+
+# ---- the step as it is used -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_whole_step_eager_and_replayed(fmt):
+    """Lengths in, attention out: tables, groups, append and shared attention, for a batch that grows by a token a step;
+    the steps run eagerly and once more as one captured graph with the lengths changed between replays."""
+    rng = np.random.default_rng(12)
+    prefix, lanes, steps = 5, 9, 3
+    start = [prefix * PAGE + int(rng.integers(0, 60)) for _ in range(lanes - 1)] + [40]
+    counts = [-(-(c + steps) // PAGE) for c in start]
+    free = iter(rng.permutation(300))  # pages of several extents
+    shared = [next(free) for _ in range(prefix)]
+    ids = [(shared if l < lanes - 1 else []) + [next(free) for _ in range(n - prefix if l < lanes - 1 else n)] for l, n in enumerate(counts)]
+    batch = Batch(fmt, ids, 12)
+    layout, storage = batch.layout, batch.storage
+    tables = ops.StepTables.for_storage(storage, lanes, max(counts))
+    runner = ops.SharedPrefixDecode(layout, 24, lanes, storage.window())
+    lane_groups, group_pages = (torch.zeros(lanes, dtype=torch.int32, device="cuda") for _ in range(2))
+    flat, offsets = dev(np.concatenate(ids).astype(np.int32)), dev(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
+    committed, rows = dev(np.array(start, np.int32)), torch.ones(lanes, dtype=torch.int32, device="cuda")
+    keys = dev(make_queries(rng, steps, lanes, HEADS, 32, DIM))
+    values = dev(make_queries(rng, steps, lanes, HEADS, DIM, 32))
+    queries = dev(make_queries(rng, steps, lanes, HEADS, 32, GROUP, DIM))
+    k, v, q = keys[0].clone(), values[0].clone(), queries[0].clone()
+    out = torch.zeros(q.shape, dtype=torch.bfloat16, device="cuda")
+    out32 = torch.zeros(q.shape, dtype=torch.float32, device="cuda")
+
+    def step(stream=None):
+        tables.build(flat, offsets, committed, rows, stream=stream)
+        ops.prefix_groups(lanes, tables.table_pointers, tables.verify_params, lane_groups, group_pages, stream=stream)
+        ops.store_verify(layout, k, v, tables.table_pointers, tables.chunk_params, batch.layer, lanes, 1, stream)
+        runner.run(q, out, tables.table_pointers, tables.verify_params, batch.layer, lane_groups, group_pages, output_f32=out32, stream=stream)
+
+    def feed(s):
+        committed.copy_(torch.tensor(start, dtype=torch.int32) + s)
+        k.copy_(keys[s]), v.copy_(values[s]), q.copy_(queries[s])
+
+    eager = []
+    for s in range(steps):
+        feed(s)
+        step()
+        tables.check()
+        runner.status()
+        assert lane_groups.cpu().tolist() == [0] * (lanes - 1) + [-1] and group_pages.cpu().tolist() == [prefix] + [0] * (lanes - 1)
+        eager.append((host16(out), out32.cpu().numpy()))
+    for extent in range(batch.host.extents):  # the pages as the device has them now
+        batch.host.bytes[extent][:] = storage.read_extent(extent)
+    host_queries = queries.cpu().view(torch.int16).numpy().view(np.uint16)
+    for s in range(steps):
+        for lane in range(lanes):
+            want, bound = batch.attend(lane, start[lane] + s, host_queries[s, lane, :, 0])
+            check_rows(eager[s][1][lane, :, 0], eager[s][0][lane, :, 0], want, bound + 2.0 ** -20 * np.abs(want).max(), f"step {s}, lane {lane}")
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    feed(0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step(stream)
+    for s in (0, 2, 1, 2):
+        feed(s)
+        out.zero_(), out32.zero_()
+        graph.replay()
+        assert np.array_equal(host16(out), eager[s][0]) and np.array_equal(out32.cpu().numpy(), eager[s][1])
+    runner.status()
+    del graph
+    runner.close()
+    batch.close()
