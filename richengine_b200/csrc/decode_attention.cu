@@ -105,7 +105,8 @@ __device__ __forceinline__ PageList lane_list(const DecodeArgs &args, uint32_t l
 struct ShapedPage {
   float cap, cap_inverse; // in the log2 domain; 0: no cap
   float slope[2];         // of this thread's two query heads, in the log2 domain
-  float distance;         // the row's position minus the page's first token
+  bool sloped;            // whether the launch has slopes
+  float distance;         // this thread's first token of the page minus the row's position
   uint32_t seen;          // bit t: token t of the page is seen
 };
 
@@ -313,6 +314,21 @@ __device__ __forceinline__ void page_softmax(const float (&sacc)[2][2][4], const
                                              const ShapedPage *shaped = nullptr) {
   float s2[2][2][2], lv[2][2];
   float local_max[2] = {-INFINITY, -INFINITY};
+  float shaped_scores[8];
+  if (Shaped) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t mt = i >> 2, half = (i >> 1) & 1u, j = i & 1u;
+      shaped_scores[i] = fmaf(sacc[mt][0][half * 2 + j] + sacc[mt][1][half * 2 + j], hfac[j], negoff[j]) *
+                         load_shared_f32(scales + (16 * mt + 8 * half + r3g) * 4);
+    }
+    if (shaped->cap > 0.0f) soft_cap(shaped_scores, shaped->cap, shaped->cap_inverse);
+    if (shaped->sloped) {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i)
+        shaped_scores[i] = fmaf(shaped->slope[i & 1u], float(16 * (i >> 2) + 8 * ((i >> 1) & 1u)) + shaped->distance, shaped_scores[i]);
+    }
+  }
 #pragma unroll
   for (uint32_t mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -326,12 +342,7 @@ __device__ __forceinline__ void page_softmax(const float (&sacc)[2][2][4], const
 #pragma unroll
       for (uint32_t j = 0; j < 2; ++j) {
         const float acc = sacc[mt][0][half * 2 + j] + sacc[mt][1][half * 2 + j];
-        float value = fmaf(acc, hfac[j], negoff[j]) * ks;
-        if (Shaped) {
-          if (shaped->cap > 0.0f) value = soft_cap(value, shaped->cap, shaped->cap_inverse);
-          value = fmaf(shaped->slope[j], float(token) - shaped->distance, value);
-        }
-        const float score = live ? value : -INFINITY;
+        const float score = live ? (Shaped ? shaped_scores[4 * mt + 2 * half + j] : fmaf(acc, hfac[j], negoff[j]) * ks) : -INFINITY;
         s2[mt][half][j] = score;
         local_max[j] = fmaxf(local_max[j], score + floor_lv);
       }
@@ -618,6 +629,7 @@ decode_int4_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
       list = lane_list(args, l, p.committed_tokens);
       shaped.cap = args.shape.cap;
       shaped.cap_inverse = args.shape.cap_inverse;
+      shaped.sloped = args.shape.slopes != nullptr;
 #pragma unroll
       for (uint32_t j = 0; j < 2; ++j)
         shaped.slope[j] = args.shape.slopes && 2 * c + j < kGroup ? __ldg(args.shape.slopes + head * kGroup + 2 * c + j) * kLog2e : 0.0f;
@@ -704,9 +716,11 @@ decode_int4_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
       uint32_t valid = kPageTokens;
       if (kShaped) { // valid only says whether the page is seen whole
         const uint32_t base = list.page(page) * kPageTokens;
-        shaped.seen = seen_tokens(base, p.committed_tokens, list.window_first, args.shape.sinks);
-        shaped.distance = float(int32_t(p.committed_tokens - base));
-        if (shaped.seen != 0xffffffffu) valid = 0;
+        shaped.distance = float(int32_t(base + r3g - p.committed_tokens));
+        if (base < list.window_first || base + kPageTokens > visible) { // few pages of a lane
+          shaped.seen = seen_tokens(base, p.committed_tokens, list.window_first, args.shape.sinks);
+          valid = 0;
+        }
       } else if (page + 1 == lane_pages) {
         valid = visible - page * kPageTokens;
       }
@@ -1008,6 +1022,7 @@ decode_bytes_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs a
       list = lane_list(args, l, p.committed_tokens);
       shaped.cap = args.shape.cap;
       shaped.cap_inverse = args.shape.cap_inverse;
+      shaped.sloped = args.shape.slopes != nullptr;
 #pragma unroll
       for (uint32_t j = 0; j < 2; ++j)
         shaped.slope[j] = args.shape.slopes && 2 * c + j < kGroup ? __ldg(args.shape.slopes + head * kGroup + 2 * c + j) * kLog2e : 0.0f;
@@ -1092,9 +1107,11 @@ decode_bytes_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs a
       uint32_t valid = kPageTokens;
       if (kShaped) { // valid only says whether the page is seen whole
         const uint32_t base = list.page(page) * kPageTokens;
-        shaped.seen = seen_tokens(base, p.committed_tokens, list.window_first, args.shape.sinks);
-        shaped.distance = float(int32_t(p.committed_tokens - base));
-        if (shaped.seen != 0xffffffffu) valid = 0;
+        shaped.distance = float(int32_t(base + r3g - p.committed_tokens));
+        if (base < list.window_first || base + kPageTokens > visible) { // few pages of a lane
+          shaped.seen = seen_tokens(base, p.committed_tokens, list.window_first, args.shape.sinks);
+          valid = 0;
+        }
       } else if (page + 1 == lane_pages) {
         valid = visible - page * kPageTokens;
       }
@@ -1343,6 +1360,7 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
       list = lane_list(args, l, p.committed_tokens);
       shaped.cap = args.shape.cap;
       shaped.cap_inverse = args.shape.cap_inverse;
+      shaped.sloped = args.shape.slopes != nullptr;
 #pragma unroll
       for (uint32_t j = 0; j < 2; ++j)
         shaped.slope[j] = args.shape.slopes && 2 * c + j < kGroup ? __ldg(args.shape.slopes + head * kGroup + 2 * c + j) * kLog2e : 0.0f;
@@ -1394,9 +1412,11 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap window_map, DecodeArgs ar
       uint32_t valid = kPageTokens;
       if (kShaped) { // valid only says whether the page is seen whole
         const uint32_t base = list.page(page) * kPageTokens;
-        shaped.seen = seen_tokens(base, p.committed_tokens, list.window_first, args.shape.sinks);
-        shaped.distance = float(int32_t(p.committed_tokens - base));
-        if (shaped.seen != 0xffffffffu) valid = 0;
+        shaped.distance = float(int32_t(base + r3g - p.committed_tokens));
+        if (base < list.window_first || base + kPageTokens > visible) { // few pages of a lane
+          shaped.seen = seen_tokens(base, p.committed_tokens, list.window_first, args.shape.sinks);
+          valid = 0;
+        }
       } else if (page + 1 == lane_pages) {
         valid = visible - page * kPageTokens;
       }

@@ -34,21 +34,34 @@ inline bool shape_arguments(const rk_score_shape *shape, ShapeArgs &out) {
   return true;
 }
 
-// cap * tanh(s / cap). tanh(u) = 1 - 2 / (e^2u + 1) loses the small u in the difference from one: its absolute error
-// of about 2^-23 is a relative one of 2^-21 only from |u| = 1/4 on. Below, the odd series u (1 - u^2/3 + 2u^4/15 -
-// 17u^6/315 + 62u^8/2835), whose next term is under 10^-8 there. So the result is good to about 10^-6 of itself
-// whatever the cap is; the hardware's tanh (2^-11) would move a score of 30 by 0.015.
-__device__ __forceinline__ float soft_cap(float s, float cap, float cap_inverse) {
-  const float u = s * cap_inverse, u2 = u * u;
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u * 2.8853900817779268f)); // e^2u
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
-  const float far = fmaf(-2.0f * cap, r, cap);
-  float near = fmaf(u2, 0.021869489f, -0.053968254f);
-  near = fmaf(u2, near, 0.13333333f);
-  near = fmaf(u2, near, -0.33333333f);
-  near = fmaf(u2 * s, near, s);
-  return u2 < 0.0625f ? near : far; // a NaN stays one
+// cap * tanh(s / cap) for N scores, tanh(u) = 1 - 2 / (e^2u + 1). The hardware's own tanh (2^-11) would move a score of 30
+// by 0.015; this form has an absolute error of about cap * 2^-22, two special-function operations per score. Caps up to
+// 256 take it as it is: under 2^-13 on a score, where the weights are rounded to 2^-11. Beyond, scores are small against
+// the cap and the difference from one loses them: below |u| = 1/4 the odd series u (1 - u^2/3 + 2u^4/15 - 17u^6/315 +
+// 62u^8/2835), whose next term is under 10^-8 there, takes over, and the result is good to about 10^-6 of itself.
+constexpr float kDirectCap = 256.0f * 1.4426950408889634f;
+template <uint32_t N> __device__ __forceinline__ void soft_cap(float (&s)[N], float cap, float cap_inverse) {
+  const float factor = cap_inverse * 2.8853900817779268f; // e^2u = 2^(2u log2 e)
+  auto far = [&](float x) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * factor));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
+    return fmaf(-2.0f * cap, r, cap);
+  };
+  if (cap <= kDirectCap) { // the same branch for the whole launch
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) s[i] = far(s[i]);
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+      const float u = s[i] * cap_inverse, u2 = u * u;
+      float near = fmaf(u2, 0.021869489f, -0.053968254f);
+      near = fmaf(u2, near, 0.13333333f);
+      near = fmaf(u2, near, -0.33333333f);
+      near = fmaf(u2 * s[i], near, s[i]);
+      s[i] = u2 < 0.0625f ? near : far(s[i]); // a NaN stays one
+    }
+  }
 }
 
 // The pages that rows at positions first_position..last_position read, as a list: page(o) for o < count. Pages before

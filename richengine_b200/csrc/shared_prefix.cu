@@ -48,13 +48,16 @@ struct Item {
   uint32_t group, first_member, leader;
 };
 
+// A group with work: its number, members and pages, and the lowest member's lane (whose table the tiles read).
+struct GroupWork { uint16_t group, members, pages, leader; };
+
 struct PlanShared {
-  uint16_t member_of[kMaxLanes]; // a lane's group, kNone: none
-  uint32_t count[kMaxLanes];     // members of a group, then (list[]) ...
-  uint32_t leader[kMaxLanes];    // its lowest member
-  uint32_t words[kMaxLanes / 32]; // members of the item's group, as bits
-  uint32_t groups, chunk, items; // groups with work; most 64-token groups of a split; items of the launch
-  uint16_t list[kMaxLanes];      // the groups with work
+  uint16_t member_of[kMaxLanes];  // a lane's group, kNone: none
+  uint32_t count[kMaxLanes];      // members of a group
+  uint32_t leader[kMaxLanes];     // its lowest member
+  GroupWork list[kMaxLanes];      // the groups with work, by leader
+  uint32_t words[kMaxLanes / 32]; // lanes as bits: leaders, then the members of the item's group
+  uint32_t groups, chunk, items;  // groups with work; most 64-token groups of a split; items of the launch
   Item item;
   uint32_t tile_lanes[kTileLanes];
 };
@@ -64,51 +67,84 @@ __device__ __forceinline__ bool lane_takes_part(rk_verify_params p) {
   return rk_verify_contract_valid(&p) && p.active_rows == 1 && p.row_capacity == 1;
 }
 __device__ __forceinline__ uint32_t tiles_of(uint32_t members) { return (members * kG + kM - 1) / kM; }
-__device__ __forceinline__ uint32_t group_pages_of(const PrefixArgs &args, const PlanShared &sh, uint32_t g) {
-  return min(args.group_pages[g], rk_pages_for(args.lane_params[sh.leader[g]].committed_tokens + 1));
-}
 __device__ __forceinline__ uint32_t units_of(uint32_t pages) { return (pages + 1) / 2; }
+// bits of the words before `word`, for a whole warp
+__device__ __forceinline__ uint32_t bits_before(const uint32_t *words, uint32_t word) {
+  const uint32_t lane = threadIdx.x % 32;
+  return __reduce_add_sync(0xffffffffu, lane < word ? uint32_t(__popc(words[lane])) : 0u);
+}
 
-// How the launch is cut, the same in every CTA: members per group, the groups with work, and the longest split for which
-// (KV heads x tiles x splits) of all groups still fit the grid. With more tiles than CTAs every tile is one item and the
-// CTAs take them in turn.
+// How the launch is cut, the same in every CTA: members per group, the groups with work, and the shortest split length for
+// which (KV heads x tiles x splits) of all groups still fit the grid. With more tiles than CTAs every tile is one item and
+// the CTAs take them in turn.
 __device__ __noinline__ void plan_launch(const PrefixArgs &args, PlanShared &sh) {
-  const uint32_t tid = threadIdx.x, lane = tid % 32, lanes = args.lanes;
+  const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32, lanes = args.lanes, words = (lanes + 31) / 32;
+  constexpr uint32_t kRounds = (kMaxLanes + kThreads - 1) / kThreads; // warps take whole words: lane i of round r is tid + r * kThreads
   for (uint32_t i = tid; i < lanes; i += kThreads) { sh.count[i] = 0; sh.leader[i] = kMaxLanes; }
   __syncthreads();
-  for (uint32_t i = tid; i < lanes; i += kThreads) {
+  uint32_t group[kRounds], pages[kRounds]; // of this thread's lanes
+#pragma unroll
+  for (uint32_t r = 0; r < kRounds; ++r) {
+    const uint32_t i = tid + r * kThreads;
+    group[r] = kNone;
+    if (i >= lanes) continue;
     const uint32_t g = args.lane_groups[i];
-    const bool member = g < lanes && args.group_pages[g] > 0 && lane_takes_part(args.lane_params[i]);
-    sh.member_of[i] = uint16_t(member ? g : kNone);
-    if (member) { atomicAdd(&sh.count[g], 1u); atomicMin(&sh.leader[g], i); }
+    const rk_verify_params p = args.lane_params[i];
+    const uint32_t shared = g < lanes ? args.group_pages[g] : 0;
+    if (shared && lane_takes_part(p)) {
+      group[r] = g;
+      pages[r] = min(shared, rk_pages_for(p.committed_tokens + 1));
+      atomicAdd(&sh.count[g], 1u);
+      atomicMin(&sh.leader[g], i);
+    }
+    sh.member_of[i] = uint16_t(group[r]);
   }
   __syncthreads();
-  if (tid < 32) {
-    uint32_t groups = 0;
-    for (uint32_t base = 0; base < lanes; base += 32) {
-      const bool work = base + lane < lanes && sh.count[base + lane] > 0;
-      const uint32_t mask = __ballot_sync(0xffffffffu, work);
-      if (work) sh.list[groups + __popc(mask & ((1u << lane) - 1u))] = uint16_t(base + lane);
-      groups += __popc(mask);
+#pragma unroll
+  for (uint32_t r = 0; r < kRounds; ++r) {
+    const uint32_t i = tid + r * kThreads;
+    if (i / 32 >= words) continue; // the whole warp
+    const uint32_t mask = __ballot_sync(0xffffffffu, group[r] != kNone && sh.leader[group[r]] == i);
+    if (lane == 0) sh.words[i / 32] = mask;
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t r = 0; r < kRounds; ++r) {
+    const uint32_t i = tid + r * kThreads;
+    if (i / 32 >= words) continue;
+    const uint32_t mask = sh.words[i / 32], at = bits_before(sh.words, i / 32) + __popc(mask & ((1u << lane) - 1u));
+    if (mask >> lane & 1u) sh.list[at] = GroupWork{uint16_t(group[r]), uint16_t(sh.count[group[r]]), uint16_t(pages[r]), uint16_t(i)};
+    if (i / 32 + 1 == words && lane == 31) sh.groups = at + (mask >> 31);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const uint32_t groups = sh.groups;
+    uint32_t units = 0, tiles = 0; // of all groups, times the KV heads
+    for (uint32_t i = lane; i < groups; i += 32) {
+      const uint32_t t = kHeads * tiles_of(sh.list[i].members);
+      tiles += t;
+      units += t * units_of(sh.list[i].pages);
     }
-    __syncwarp();
+    units = __reduce_add_sync(0xffffffffu, units);
+    tiles = __reduce_add_sync(0xffffffffu, tiles);
     auto items_for = [&](uint32_t chunk) {
       uint32_t sum = 0;
-      for (uint32_t i = lane; i < groups; i += 32) {
-        const uint32_t g = sh.list[i];
-        sum += kHeads * tiles_of(sh.count[g]) * ((units_of(group_pages_of(args, sh, g)) + chunk - 1) / chunk);
-      }
+      for (uint32_t i = lane; i < groups; i += 32)
+        sum += kHeads * tiles_of(sh.list[i].members) * ((units_of(sh.list[i].pages) + chunk - 1) / chunk);
       return __reduce_add_sync(0xffffffffu, sum);
     };
-    uint32_t low = kLeastUnits, high = units_of(rk_pages_for(RK_MAX_PHYSICAL_TOKENS)); // the least chunk that fits, if any does
-    if (groups && items_for(high) <= gridDim.x) {
+    // items(chunk) <= units / chunk + tiles, and >= units / chunk: the shortest chunk that fits lies between these two
+    uint32_t high = units_of(rk_pages_for(RK_MAX_PHYSICAL_TOKENS));
+    if (tiles < gridDim.x) {
+      high = max(kLeastUnits, units / (gridDim.x - tiles) + 1);
+      uint32_t low = max(kLeastUnits, (units + gridDim.x - 1) / gridDim.x);
       while (low < high) {
         const uint32_t middle = (low + high) / 2;
         if (items_for(middle) <= gridDim.x) high = middle; else low = middle + 1;
       }
     }
-    const uint32_t items = groups ? items_for(high) : 0;
-    if (lane == 0) { sh.groups = groups; sh.chunk = high; sh.items = items; }
+    const uint32_t items = items_for(high);
+    if (lane == 0) { sh.chunk = high; sh.items = items; }
   }
   __syncthreads();
 }
@@ -120,10 +156,9 @@ __device__ __noinline__ void find_item(const PrefixArgs &args, PlanShared &sh, u
     uint32_t before = 0, rows = 0;
     for (uint32_t base = 0; base < sh.groups; base += 32) {
       const bool live = base + lane < sh.groups;
-      const uint32_t g = live ? sh.list[base + lane] : 0;
-      const uint32_t pages = live ? group_pages_of(args, sh, g) : 0, members = live ? sh.count[g] : 0;
-      const uint32_t splits = (units_of(pages) + sh.chunk - 1) / sh.chunk, tiles = tiles_of(members);
-      const uint32_t items = kHeads * tiles * splits, group_rows = members * kG;
+      const GroupWork work = live ? sh.list[base + lane] : GroupWork{0, 0, 0, 0};
+      const uint32_t units = units_of(work.pages), splits = (units + sh.chunk - 1) / sh.chunk, tiles = tiles_of(work.members);
+      const uint32_t items = kHeads * tiles * splits, group_rows = work.members * kG;
       uint32_t items_up = items, rows_up = kHeads * splits * group_rows;
 #pragma unroll
       for (uint32_t o = 1; o < 32; o <<= 1) {
@@ -133,7 +168,7 @@ __device__ __noinline__ void find_item(const PrefixArgs &args, PlanShared &sh, u
       const uint32_t found = __ballot_sync(0xffffffffu, live && index < before + items_up);
       if (found) {
         if (lane == uint32_t(__ffs(found) - 1)) {
-          const uint32_t within = index - (before + items_up - items), units = units_of(pages);
+          const uint32_t within = index - (before + items_up - items);
           Item &item = sh.item;
           item.head = within % kHeads;
           item.tile = within / kHeads % tiles;
@@ -142,9 +177,9 @@ __device__ __noinline__ void find_item(const PrefixArgs &args, PlanShared &sh, u
           item.group_rows = group_rows;
           item.row_base = rows + rows_up - kHeads * splits * group_rows;
           item.page_begin = 2 * (units * item.split / splits);
-          item.page_end = min(pages, 2 * (units * (item.split + 1) / splits));
-          item.group = g;
-          item.leader = sh.leader[g];
+          item.page_end = min(uint32_t(work.pages), 2 * (units * (item.split + 1) / splits));
+          item.group = work.group;
+          item.leader = work.leader;
           item.first_member = item.tile * kM / kG;
         }
         break;
@@ -162,8 +197,7 @@ __device__ __noinline__ void find_item(const PrefixArgs &args, PlanShared &sh, u
   }
   __syncthreads();
   for (uint32_t w = warp; w < (lanes + 31) / 32; w += kThreads / 32) {
-    const uint32_t earlier = __reduce_add_sync(0xffffffffu, lane < w ? uint32_t(__popc(sh.words[lane])) : 0u);
-    const uint32_t rank = earlier + __popc(sh.words[w] & ((1u << lane) - 1u));
+    const uint32_t rank = bits_before(sh.words, w) + __popc(sh.words[w] & ((1u << lane) - 1u));
     if ((sh.words[w] >> lane & 1u) && rank >= sh.item.first_member && rank < sh.item.first_member + kTileLanes)
       sh.tile_lanes[rank - sh.item.first_member] = 32 * w + lane;
   }
@@ -261,10 +295,10 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap head_map, PrefixArgs ar
           for (uint32_t i = 0; i < 4; ++i)
             amax = fmaxf(amax, fmaxf(fabsf(bf16_bits_to_float(words[i] & 0xffffu)), fabsf(bf16_bits_to_float(words[i] >> 16))));
         }
-        ctl.exchange[1][my_row][part] = amax;
+        ctl.exchange[1][part][my_row] = amax;
         asm volatile("bar.sync %0, %1;" ::"r"(1u + quarter), "n"(32 * kRowThreads) : "memory");
 #pragma unroll
-        for (uint32_t i = 0; i < kRowThreads; ++i) amax = fmaxf(amax, ctl.exchange[1][my_row][i]);
+        for (uint32_t i = 0; i < kRowThreads; ++i) amax = fmaxf(amax, ctl.exchange[1][i][my_row]);
         if (amax >= 8192.0f) exponent = ilogbf(amax) - 12;
       }
       const float down = ldexpf(1.0f, -exponent);
@@ -300,7 +334,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap head_map, PrefixArgs ar
         for (uint32_t i = 0; i < 4; ++i) columns[c * 4 + i] = __uint_as_float(chunk[i]);
       }
       tmem_store32(tmem_q + ((quarter * 32u) << 16) + column, columns);
-      ctl.exchange[0][my_row][part] = q_sum;
+      ctl.exchange[0][part][my_row] = q_sum;
     }
     tmem_fence_before();
     __syncthreads();
@@ -308,7 +342,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap head_map, PrefixArgs ar
     if (tid < kM) {
       float total = 0.0f;
 #pragma unroll
-      for (uint32_t i = 0; i < kRowThreads; ++i) total += ctl.exchange[0][tid][i];
+      for (uint32_t i = 0; i < kRowThreads; ++i) total += ctl.exchange[0][i][tid];
       ctl.q_sums[tid] = total;
     }
     __syncthreads();
@@ -398,17 +432,17 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap head_map, PrefixArgs ar
         if (e < kGroupTokens) {
           if (n >= kScaleStages) barrier_wait(&ctl.scale_free[n % kScaleStages], n / kScaleStages - 1, error);
           const uint32_t token = Expand<Format>::token_of(e);
-          float4 triple = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          float3 triple = make_float3(0.0f, 0.0f, 0.0f);
           if (valid.holds(token)) {
             if (Kind::kScales) {
               const float ks = reinterpret_cast<const float *>(raw + kRawScaleOffset)[token];
               const float vs = fmaxf(reinterpret_cast<const float *>(raw + kRawScaleOffset)[64 + token], 9.094947e-13f); // 2^-40
-              triple = make_float4(ks, log2_fast(vs), __fdividef(0.015625f, vs), 0.0f);
+              triple = make_float3(ks, log2_fast(vs), __fdividef(0.015625f, vs));
             } else {
-              triple = make_float4(1.0f, 0.0f, 0.015625f, 0.0f);
+              triple = make_float3(1.0f, 0.0f, 0.015625f);
             }
           }
-          ctl.scales[n % kScaleStages][e] = triple;
+          ctl.scales[n % kScaleStages].put(e, triple.x, triple.y, triple.z);
         }
         if (round) barrier_wait(&ctl.k_free[team], round - 1, error);
         Expand<Format>::template keys<kExpandThreads>(raw, k_ptr + team * kKBytes, e);
@@ -436,46 +470,29 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap head_map, PrefixArgs ar
       float row_max = -1.0e30f, row_sum = 0.0f; // row_sum: this thread's tokens only
       for (uint32_t g = 0; g < groups; ++g) {
         const uint32_t n = done + g, b = n & 1u, first = page_begin + 2 * g, base = first * kPageTokens;
-        uint32_t seen_first = seen_tokens(base, position, row_window, kShaped ? args.shape.sinks : 0);
-        uint32_t seen_second = first + 1 < page_end ? seen_tokens(base + kPageTokens, position, row_window, kShaped ? args.shape.sinks : 0) : 0u;
-        if (!real) seen_first = seen_second = 0xffffffffu; // a row without a lane holds a zero query: what it sees is of no interest
-        const bool whole = __all_sync(0xffffffffu, (seen_first & seen_second) == 0xffffffffu);
-        const float4 *triples = ctl.scales[n % kScaleStages] + part * kRowTokens;
+        const GroupView view{base, base + kPageTokens, first + 1 < page_end};
+        const ScaleStage &stage = ctl.scales[n % kScaleStages];
         barrier_wait(&ctl.s_full[b], n >> 1, error);
         tmem_fence_after();
         float scores[kRowTokens];
         tmem_load_scores(tmem_s + b * 64 + lane_address + part * kRowTokens, scores);
         float group_max = -INFINITY;
-        if (!kShaped && whole) {
-#pragma unroll
-          for (uint32_t i = 0; i < kRowTokens; ++i) {
-            const float4 triple = triples[i];
-            scores[i] = fmaf(scores[i], row_factor, row_offset) * triple.x + triple.y; // score + log2(value scale)
-            group_max = fmaxf(group_max, scores[i]);
-          }
+        if (kShaped) {
+          shape_scores<kRowTokens, kPermuted>(scores, stage, part * kRowTokens, row_factor, row_offset, part_token, args.shape, slope, view, position);
         } else {
-          const float distance = float(int32_t(position - base));
-          const bool capped = kShaped && args.shape.cap > 0.0f;
-#pragma unroll
-          for (uint32_t i = 0; i < kRowTokens; ++i) {
-            const uint32_t local = (kPermuted ? 8 * (i & 7u) + (i >> 3) : i) + part_token;
-            const float4 triple = triples[i];
-            float s = fmaf(scores[i], row_factor, row_offset) * triple.x;
-            if (capped) s = soft_cap(s, args.shape.cap, args.shape.cap_inverse);
-            s = (kShaped ? fmaf(slope, float(local) - distance, s) : s) + triple.y;
-            const bool admitted = whole || (((local < kPageTokens ? seen_first : seen_second) >> (local & 31u)) & 1u);
-            scores[i] = admitted ? s : -INFINITY;
-            group_max = fmaxf(group_max, scores[i]);
-          }
+          scale_scores(scores, stage, part * kRowTokens, row_factor, row_offset);
         }
+        mask_scores<kRowTokens, kPermuted>(scores, part_token, view, position, row_window, kShaped ? args.shape.sinks : 0, real);
+#pragma unroll
+        for (uint32_t i = 0; i < kRowTokens; ++i) group_max = fmaxf(group_max, scores[i]);
         // the row's other parts; past this barrier every part holds its scores in registers, so the probabilities may
         // overwrite the first 32 columns of the buffer
-        ctl.exchange[b][my_row][part] = group_max;
+        ctl.exchange[b][part][my_row] = group_max;
         tmem_fence_before();
         asm volatile("bar.sync %0, %1;" ::"r"(1u + quarter), "n"(32 * kRowThreads) : "memory");
         tmem_fence_after();
 #pragma unroll
-        for (uint32_t i = 0; i < kRowThreads; ++i) group_max = fmaxf(group_max, ctl.exchange[b][my_row][i]);
+        for (uint32_t i = 0; i < kRowThreads; ++i) group_max = fmaxf(group_max, ctl.exchange[b][i][my_row]);
         // the reference exponent only moves when the maximum grew by more than 2^8: fp16 probabilities stay below 2^14
         const bool grow = group_max > row_max + 8.0f;
         float scale = 1.0f;
@@ -485,15 +502,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap head_map, PrefixArgs ar
           row_sum *= scale;
         }
         const float exponent_base = row_max - 6.0f;
+        weigh_scores(scores, stage, part * kRowTokens, exponent_base, row_sum); // row_sum: of 2^(score - row_max)
         uint32_t packed[kRowTokens / 2], packed_low[Kind::kBf16 ? kRowTokens / 2 : 1];
 #pragma unroll
         for (uint32_t c = 0; c < kRowTokens / 2; ++c) {
-          float w[2];
-#pragma unroll
-          for (uint32_t h = 0; h < 2; ++h) {
-            w[h] = exp2_fast(scores[2 * c + h] - exponent_base);     // 0 for a masked token
-            row_sum = fmaf(w[h], triples[2 * c + h].z, row_sum);     // 2^(score - row_max)
-          }
+          const float w[2] = {scores[2 * c], scores[2 * c + 1]};
           if (Kind::kBf16) { // a high and a low bf16 part: 16 bits of the probability
             packed[c] = pack_bfloat2(w[0], w[1]);
             packed_low[c] = pack_bfloat2(w[0] - __uint_as_float(packed[c] << 16), w[1] - __uint_as_float(packed[c] & 0xffff0000u));
@@ -537,12 +550,12 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap head_map, PrefixArgs ar
             *reinterpret_cast<float4 *>(out + c * 32 + i) = make_float4(o[i] * 0.015625f, o[i + 1] * 0.015625f, o[i + 2] * 0.015625f, o[i + 3] * 0.015625f);
         }
       }
-      ctl.exchange[(last + 1) & 1u][my_row][part] = row_sum;
+      ctl.exchange[(last + 1) & 1u][part][my_row] = row_sum;
       asm volatile("bar.sync %0, %1;" ::"r"(1u + quarter), "n"(32 * kRowThreads) : "memory");
       if (part == 0 && real) {
         float total = 0.0f;
 #pragma unroll
-        for (uint32_t i = 0; i < kRowThreads; ++i) total += ctl.exchange[(last + 1) & 1u][my_row][i];
+        for (uint32_t i = 0; i < kRowThreads; ++i) total += ctl.exchange[(last + 1) & 1u][i][my_row];
         args.statistics[row * 2] = failed ? -INFINITY : row_max * kLn2;
         args.statistics[row * 2 + 1] = failed ? 0.0f : total;
       }

@@ -218,7 +218,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
       }
       tmem_store32(tmem_q + ((quarter * 32u) << 16) + column, columns);
     }
-    ctl.exchange[0][row][part] = q_sum;
+    ctl.exchange[0][part][row] = q_sum;
   }
   tmem_fence_before();
   __syncthreads();
@@ -226,7 +226,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
   if (tid < kM) {
     float total = 0.0f;
 #pragma unroll
-    for (uint32_t i = 0; i < kRowThreads; ++i) total += ctl.exchange[0][tid][i];
+    for (uint32_t i = 0; i < kRowThreads; ++i) total += ctl.exchange[0][i][tid];
     ctl.q_sums[tid] = total;
   }
   __syncthreads();
@@ -337,8 +337,10 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
       // positions of the group whose tokens exist: the split may end inside the group, the lane inside the page
       const auto valid = [&] {
         if constexpr (kShaped) {
-          auto seen = [&](uint32_t o) { return o < page_end ? seen_tokens(list.page(o) * kPageTokens, visible - 1, list.window_first, args.shape.sinks) : 0u; };
-          return ValidBits{uint64_t(seen(first)) | uint64_t(seen(first + 1)) << 32};
+          const GroupView view{list.page(first) * kPageTokens, list.page(first + 1) * kPageTokens, first + 1 < page_end};
+          if (view.whole(visible - 1, list.window_first)) return ValidBits{~uint64_t(0)};
+          return ValidBits{uint64_t(view.seen_first(visible - 1, list.window_first, args.shape.sinks)) |
+                           uint64_t(view.seen_second(visible - 1, list.window_first, args.shape.sinks)) << 32};
         } else {
           return ValidBelow{min(min(2u, page_end - first) * kPageTokens, visible - first * kPageTokens)};
         }
@@ -350,17 +352,17 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
       if (e < kGroupTokens) {
         if (g >= kScaleStages) barrier_wait(&ctl.scale_free[g % kScaleStages], g / kScaleStages - 1, error);
         const uint32_t token = Expand<Format>::token_of(e);
-        float4 triple = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float3 triple = make_float3(0.0f, 0.0f, 0.0f);
         if (valid.holds(token)) {
           if (Kind::kScales) {
             const float ks = reinterpret_cast<const float *>(raw + kRawScaleOffset)[token];
             const float vs = fmaxf(reinterpret_cast<const float *>(raw + kRawScaleOffset)[64 + token], 9.094947e-13f); // 2^-40
-            triple = make_float4(ks, log2_fast(vs), __fdividef(0.015625f, vs), 0.0f);
+            triple = make_float3(ks, log2_fast(vs), __fdividef(0.015625f, vs));
           } else {
-            triple = make_float4(1.0f, 0.0f, 0.015625f, 0.0f);
+            triple = make_float3(1.0f, 0.0f, 0.015625f);
           }
         }
-        ctl.scales[g % kScaleStages][e] = triple;
+        ctl.scales[g % kScaleStages].put(e, triple.x, triple.y, triple.z);
       }
       if (round) barrier_wait(&ctl.k_free[b], round - 1, error);
       Expand<Format>::template keys<kExpandThreads>(raw, k_ptr + b * kKBytes, e);
@@ -384,6 +386,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
     const uint32_t causal_limit = min(visible, p.committed_tokens + min(query_row, p.active_rows - 1) + 1);
     const uint32_t tree_mask = kTree && query_row < p.row_capacity ? row_masks[query_row] : 0u;
     const uint32_t row_position = p.committed_tokens + min(query_row, p.active_rows - 1);
+    const uint32_t row_window = kShaped && args.shape.window && row_position + 1 > args.shape.window ? row_position + 1 - args.shape.window : 0;
     const float slope = kShaped && args.shape.slopes && my_row < kRealRows ? __ldg(args.shape.slopes + kv_head * kG + my_row % kG) * kLog2e : 0.0f;
     const uint32_t lane_address = (quarter * 32u) << 16;
     constexpr uint32_t kOutColumns = kD / kRowThreads; // columns of O this thread rescales and writes out
@@ -399,7 +402,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
       constexpr bool kPermuted = Format == RK_FORMAT_INT4;
       const uint32_t part_token = kPermuted ? (kRowTokens / 8) * part : kRowTokens * part;
       const int32_t bound = int32_t(limit) - int32_t(part_token);
-      const float4 *triples = ctl.scales[g % kScaleStages] + part * kRowTokens;
+      const ScaleStage &stage = ctl.scales[g % kScaleStages];
       barrier_wait(&ctl.s_full[b], g >> 1, error);
       tmem_fence_after();
       float scores[kRowTokens];
@@ -407,35 +410,18 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
 
       float group_max = -INFINITY;
       if constexpr (kShaped) {
-        // tokens of position kRowTokens*part + i: base of its page + offset; the two pages of a group need not be neighbours
-        const uint32_t first_base = list.page(first) * kPageTokens;
-        const uint32_t second_base = first + 1 < page_end ? list.page(first + 1) * kPageTokens : first_base + kPageTokens;
-        const uint32_t row_window = args.shape.window && row_position + 1 > args.shape.window ? row_position + 1 - args.shape.window : 0;
-        uint32_t seen_first = seen_tokens(first_base, row_position, row_window, args.shape.sinks);
-        uint32_t seen_second = present > kPageTokens ? seen_tokens(second_base, row_position, row_window, args.shape.sinks) : 0u;
-        const bool capped = args.shape.cap > 0.0f;
-        const float first_distance = float(int32_t(row_position - first_base)), second_distance = float(int32_t(row_position - second_base)) + 32.0f;
-        // a whole warp's rows usually see the whole group: the tests of single tokens are left out then
-        const bool whole = __all_sync(0xffffffffu, (seen_first & seen_second) == 0xffffffffu);
+        // the two pages of a group need not be neighbours
+        const GroupView view{list.page(first) * kPageTokens, list.page(first + 1) * kPageTokens, present > kPageTokens};
+        shape_scores<kRowTokens, kPermuted>(scores, stage, part * kRowTokens, row_factor, row_offset, part_token, args.shape, slope, view, row_position);
+        mask_scores<kRowTokens, kPermuted>(scores, part_token, view, row_position, row_window, args.shape.sinks);
 #pragma unroll
-        for (uint32_t i = 0; i < kRowTokens; ++i) {
-          const uint32_t local = (kPermuted ? 8 * (i & 7u) + (i >> 3) : i) + part_token;
-          const float4 triple = triples[i];
-          float s = fmaf(scores[i], row_factor, row_offset) * triple.x;
-          if (capped) s = soft_cap(s, args.shape.cap, args.shape.cap_inverse);
-          s = fmaf(slope, float(local) - (local < kPageTokens ? first_distance : second_distance), s) + triple.y;
-          const bool admitted = whole || (((local < kPageTokens ? seen_first : seen_second) >> (local & 31u)) & 1u);
-          scores[i] = admitted ? s : -INFINITY;
-          group_max = fmaxf(group_max, scores[i]);
-        }
+        for (uint32_t i = 0; i < kRowTokens; ++i) group_max = fmaxf(group_max, scores[i]);
       } else if (!kTree && limit >= kGroupTokens) { // every token of the group is admitted (all but the last groups of a lane)
+        scale_scores(scores, stage, part * kRowTokens, row_factor, row_offset);
 #pragma unroll
-        for (uint32_t i = 0; i < kRowTokens; ++i) {
-          const float4 triple = triples[i];
-          scores[i] = fmaf(scores[i], row_factor, row_offset) * triple.x + triple.y; // score + log2(value scale)
-          group_max = fmaxf(group_max, scores[i]);
-        }
+        for (uint32_t i = 0; i < kRowTokens; ++i) group_max = fmaxf(group_max, scores[i]);
       } else {
+        scale_scores(scores, stage, part * kRowTokens, row_factor, row_offset);
 #pragma unroll
         for (uint32_t i = 0; i < kRowTokens; ++i) {
           const int32_t local = kPermuted ? int32_t(8 * (i & 7u) + (i >> 3)) : int32_t(i);
@@ -444,20 +430,18 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
             const uint32_t token = token_base + uint32_t(local) + part_token;
             admitted = admitted && (token < p.committed_tokens || (token < visible && ((tree_mask >> (token - p.committed_tokens)) & 1u)));
           }
-          const float4 triple = triples[i];
-          const float s = fmaf(scores[i], row_factor, row_offset) * triple.x + triple.y;
-          scores[i] = admitted ? s : -INFINITY;
+          if (!admitted) scores[i] = -INFINITY;
           group_max = fmaxf(group_max, scores[i]);
         }
       }
       // the row's other parts; past this barrier every part holds its scores in registers, so the
       // probabilities may overwrite the first 32 columns of the buffer
-      ctl.exchange[b][my_row][part] = group_max;
+      ctl.exchange[b][part][my_row] = group_max;
       tmem_fence_before();
       asm volatile("bar.sync %0, %1;" ::"r"(1u + quarter), "n"(32 * kRowThreads) : "memory");
       tmem_fence_after();
 #pragma unroll
-      for (uint32_t i = 0; i < kRowThreads; ++i) group_max = fmaxf(group_max, ctl.exchange[b][my_row][i]);
+      for (uint32_t i = 0; i < kRowThreads; ++i) group_max = fmaxf(group_max, ctl.exchange[b][i][my_row]);
       // Lazy rescale: the reference exponent only moves when the maximum grew by more than 2^8, so the
       // fp16 probabilities stay below 2^(8+6); rows of a warp move together (collective TMEM access).
       const bool grow = group_max > row_max + 8.0f;
@@ -470,15 +454,11 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
       const float exponent_base = row_max - 6.0f;
       // bf16 probabilities alone carry 8 bits: they travel as a high and a low bf16 part (two contractions), which
       // restores 16 bits; the low parts take the second half of the S buffer
+      weigh_scores(scores, stage, part * kRowTokens, exponent_base, row_sum); // row_sum: of 2^(score - row_max)
       uint32_t packed[kRowTokens / 2], packed_low[Kind::kBf16 ? kRowTokens / 2 : 1];
 #pragma unroll
       for (uint32_t c = 0; c < kRowTokens / 2; ++c) {
-        float w[2];
-#pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
-          w[h] = exp2_fast(scores[2 * c + h] - exponent_base);     // 0 for a masked token
-          row_sum = fmaf(w[h], triples[2 * c + h].z, row_sum);     // 2^(score - row_max)
-        }
+        const float w[2] = {scores[2 * c], scores[2 * c + 1]};
         if (Kind::kBf16) {
           packed[c] = pack_bfloat2(w[0], w[1]);
           packed_low[c] = pack_bfloat2(w[0] - __uint_as_float(packed[c] << 16), w[1] - __uint_as_float(packed[c] & 0xffff0000u));
@@ -527,12 +507,12 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
           *reinterpret_cast<float4 *>(out + c * 32 + i) = make_float4(o[i] * 0.015625f, o[i + 1] * 0.015625f, o[i + 2] * 0.015625f, o[i + 3] * 0.015625f);
       }
     }
-    ctl.exchange[groups & 1u][my_row][part] = row_sum;
+    ctl.exchange[groups & 1u][part][my_row] = row_sum;
     asm volatile("bar.sync %0, %1;" ::"r"(1u + quarter), "n"(32 * kRowThreads) : "memory");
     if (part == 0 && row_exists) {
       float total = 0.0f;
 #pragma unroll
-      for (uint32_t i = 0; i < kRowThreads; ++i) total += ctl.exchange[groups & 1u][my_row][i];
+      for (uint32_t i = 0; i < kRowThreads; ++i) total += ctl.exchange[groups & 1u][i][my_row];
       float *stats = args.statistics + (slot * kSlotRows + slot_row) * 2;
       stats[0] = failed ? -INFINITY : row_max * kLn2;
       stats[1] = failed ? 0.0f : total;

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "score_shape.cuh"
 #include "window.cuh"
 
 #include <cuda_bf16.h>
@@ -70,6 +71,20 @@ template <uint32_t Format> __host__ __device__ constexpr uint32_t tile_bytes() {
 // tensor-memory columns
 constexpr uint32_t kTmemO = 0, kTmemS = 256, kTmemQ = 384; // S twice (64 columns each); P(g) overwrites the first half of S(g)
 
+// The per-token scales of a group, laid out for a softmax thread's neighbouring positions: two tokens' {key scale pair, log2
+// value scale pair} in one 16-byte word (operands of packed fp32 arithmetic), the factors of four tokens in another. Every
+// thread of a row reads the same words, a wavefront each: 12 of them for 16 tokens instead of 32.
+struct ScaleStage {
+  float4 pairs[kGroupTokens / 2];   // {key scale, key scale, log2 value scale, log2 value scale}
+  float4 factors[kGroupTokens / 4]; // 2^-6 / value scale
+  __device__ __forceinline__ void put(uint32_t position, float key_scale, float value_log, float factor) {
+    float *pair = reinterpret_cast<float *>(&pairs[position >> 1]) + (position & 1u);
+    pair[0] = key_scale;
+    pair[2] = value_log;
+    reinterpret_cast<float *>(factors)[position] = factor;
+  }
+};
+
 struct Control {
   uint64_t raw_full[kMaxRawStages], raw_free[kMaxRawStages];
   uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], p_free[2], scale_free[kScaleStages];
@@ -78,8 +93,8 @@ struct Control {
   uint32_t error;
   uint32_t spin_limit; // directly after `error`: barrier_wait reads it through the error pointer
   float q_sums[kM];
-  float exchange[2][kM][kRowThreads]; // the part-row maxima of a group (and, at the end, the part-row sums)
-  float4 scales[kScaleStages][kGroupTokens]; // {key scale, log2 value scale, 2^-6 / value scale, -}
+  float exchange[2][kRowThreads][kM]; // the part-row maxima of a group (and, at the end, the part-row sums); a warp's rows side by side
+  ScaleStage scales[kScaleStages];
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return uint32_t(__cvta_generic_to_shared(p)); }
@@ -411,5 +426,124 @@ template <> struct Expand<RK_FORMAT_BF16> {
     }
   }
 };
+
+// ---- a softmax thread's N scores of a 64-token group ----------------------------------------------------------------
+// Two fp32 operations in one instruction, each rounded as on its own.
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
+  float2 r;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+  float2 r;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+// Accumulators to scores + log2(value scale); `position` is the thread's first of the group.
+template <uint32_t N>
+__device__ __forceinline__ void scale_scores(float (&scores)[N], const ScaleStage &stage, uint32_t position, float row_factor, float row_offset) {
+  const float2 factor = make_float2(row_factor, row_factor), offset = make_float2(row_offset, row_offset);
+#pragma unroll
+  for (uint32_t i = 0; i < N; i += 2) {
+    const float4 pair = stage.pairs[(position + i) >> 1];
+    const float2 s = fma_pair(fma_pair(make_float2(scores[i], scores[i + 1]), factor, offset), make_float2(pair.x, pair.y), make_float2(pair.z, pair.w));
+    scores[i] = s.x;
+    scores[i + 1] = s.y;
+  }
+}
+// Scores to weights 2^(score - base); `sum` takes each weight times its token's factor, in order.
+template <uint32_t N>
+__device__ __forceinline__ void weigh_scores(float (&scores)[N], const ScaleStage &stage, uint32_t position, float base, float &sum) {
+#pragma unroll
+  for (uint32_t i = 0; i < N; i += 4) {
+    const float4 factor = stage.factors[(position + i) >> 2];
+    const float2 low = add_pair(make_float2(scores[i], scores[i + 1]), make_float2(-base, -base));
+    const float2 high = add_pair(make_float2(scores[i + 2], scores[i + 3]), make_float2(-base, -base));
+    scores[i] = exp2_fast(low.x); scores[i + 1] = exp2_fast(low.y); // 0 for a masked token
+    scores[i + 2] = exp2_fast(high.x); scores[i + 3] = exp2_fast(high.y);
+    sum = fmaf(scores[i], factor.x, sum); sum = fmaf(scores[i + 1], factor.y, sum);
+    sum = fmaf(scores[i + 2], factor.z, sum); sum = fmaf(scores[i + 3], factor.w, sum);
+  }
+}
+// Score i belongs to token part_token + local_token<...>(i) of the group: the first page's tokens below 32, the second's
+// above. Which page that is, is known at compile time where the tokens are permuted and by the thread's part elsewhere.
+template <bool kPermuted> __device__ __forceinline__ constexpr uint32_t local_token(uint32_t i) { return kPermuted ? 8 * (i & 7u) + (i >> 3) : i; }
+
+// What a row (or all rows of a tile: the last one's position, the first one's window) sees of a group's two pages, which
+// begin at tokens `first` and `second`.
+struct GroupView {
+  uint32_t first, second;
+  bool both; // the group has a second page
+  // every token, by their positions alone (the sinks aside)
+  __device__ __forceinline__ bool whole(uint32_t position, uint32_t window_first) const {
+    return both && first >= window_first && second + (kPageTokens - 1) <= position;
+  }
+  __device__ __forceinline__ uint32_t seen_first(uint32_t position, uint32_t window_first, uint32_t sinks) const {
+    return seen_tokens(first, position, window_first, sinks);
+  }
+  __device__ __forceinline__ uint32_t seen_second(uint32_t position, uint32_t window_first, uint32_t sinks) const {
+    return both ? seen_tokens(second, position, window_first, sinks) : 0u;
+  }
+};
+
+// Scores of unseen tokens become -infinity. A warp's rows usually see the whole group: nothing is worked out or tested then
+// (the bits cost about as many instructions as the scores of a thread).
+template <uint32_t N, bool kPermuted>
+__device__ __forceinline__ void mask_scores(float (&scores)[N], uint32_t part_token, const GroupView &view, uint32_t position,
+                                            uint32_t window_first, uint32_t sinks, bool real = true) {
+  if (__all_sync(0xffffffffu, !real || view.whole(position, window_first))) return;
+  const uint32_t seen_first = view.seen_first(position, window_first, sinks), seen_second = view.seen_second(position, window_first, sinks);
+  static_assert(kPermuted || N <= kPageTokens, "an unpermuted part lies in one page");
+  const uint32_t mine = part_token < kPageTokens ? seen_first : seen_second;
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) {
+    const uint32_t bits = kPermuted ? (local_token<kPermuted>(i) < kPageTokens ? seen_first : seen_second) : mine;
+    if (!((bits >> ((local_token<kPermuted>(i) + part_token) & 31u)) & 1u)) scores[i] = -INFINITY;
+  }
+}
+
+// Accumulators to scores + log2(value scale) through a shape, without the mask. Each stage is one branch for the launch.
+template <uint32_t N, bool kPermuted>
+__device__ __forceinline__ void shape_scores(float (&scores)[N], const ScaleStage &stage, uint32_t first_position, float row_factor,
+                                             float row_offset, uint32_t part_token, const ShapeArgs &shape, float slope,
+                                             const GroupView &view, uint32_t position) {
+  if (shape.cap == 0.0f && !shape.slopes) {
+    scale_scores(scores, stage, first_position, row_factor, row_offset);
+    return;
+  }
+  const float2 factor = make_float2(row_factor, row_factor), offset = make_float2(row_offset, row_offset);
+#pragma unroll
+  for (uint32_t i = 0; i < N; i += 2) {
+    const float2 keys = *reinterpret_cast<const float2 *>(&stage.pairs[(first_position + i) >> 1]);
+    const float2 s = mul_pair(fma_pair(make_float2(scores[i], scores[i + 1]), factor, offset), keys);
+    scores[i] = s.x;
+    scores[i + 1] = s.y;
+  }
+  if (shape.cap > 0.0f) soft_cap(scores, shape.cap, shape.cap_inverse);
+  if (shape.slopes) {
+    const float first = float(int32_t(view.first - position + part_token)), second = float(int32_t(view.second - position + part_token - kPageTokens));
+    const float mine = part_token < kPageTokens ? first : second;
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+      const float origin = kPermuted ? (local_token<kPermuted>(i) < kPageTokens ? first : second) : mine;
+      scores[i] = fmaf(slope, origin + float(local_token<kPermuted>(i)), scores[i]);
+    }
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < N; i += 2) {
+    const float2 logs = *(reinterpret_cast<const float2 *>(&stage.pairs[(first_position + i) >> 1]) + 1);
+    const float2 s = add_pair(make_float2(scores[i], scores[i + 1]), logs);
+    scores[i] = s.x;
+    scores[i + 1] = s.y;
+  }
+}
 
 } // namespace rk::tile
