@@ -486,7 +486,10 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
     }
 
     // ---- partial output: row i of O, un-normalised; statistics {reference exponent, sum} -------------------
-    barrier_wait(&ctl.v_free[(groups - 1) % kTileStages], (groups - 1) / kTileStages, error);
+    // Every contraction into O has landed when the last group's has. p_free says so without doubt: its completion before
+    // that one, two groups earlier, preceded the last scores. v_free of a format with one operand stage may still be two
+    // completions behind here, which a parity wait takes for done.
+    barrier_wait(&ctl.p_free[(groups - 1) & 1u], (groups - 1) >> 1, error);
     tmem_fence_after();
     const bool failed = *error != 0;
     // verify: one slot of kRealRows fused rows per (lane, head, split); prefill: one slot of 48 fused rows per tile
