@@ -59,7 +59,9 @@ template <uint32_t N> __device__ __forceinline__ void soft_cap(float (&s)[N], fl
       near = fmaf(u2, near, 0.13333333f);
       near = fmaf(u2, near, -0.33333333f);
       near = fmaf(u2 * s[i], near, s[i]);
-      s[i] = u2 < 0.0625f ? near : far(s[i]); // a NaN stays one
+      s[i] = far(s[i]);
+      // a select, not a branch: 64 branches would keep every score's both sides alive (a NaN stays one)
+      asm("{\n.reg .pred p;\nsetp.lt.f32 p, %2, 0f3D800000;\nselp.f32 %0, %1, %0, p;\n}" : "+f"(s[i]) : "f"(near), "f"(u2));
     }
   }
 }

@@ -35,7 +35,6 @@
 // Every mbarrier wait is bounded and gives up at once after any wait failed; TMEM is released on
 // every path.
 #include "common.cuh"
-#include "score_shape.cuh"
 #include "window_tile.cuh"
 
 #include <type_traits>
@@ -59,15 +58,13 @@ struct VerifyArgs {
   // prefill launches (grid z = 8-row tile of the chunk): the sequence's table and parameters instead of per-lane ones
   const rk_page_entry *prefill_table;
   rk_prefill_params prefill;
-  ShapeArgs shape; // shaped launches (kShaped) only
 };
 
 // kPrefill: the CTA's window is `Rows` consecutive rows of a prefill chunk (prefill/paged_attention.metal:7-67), starting
 // at row Rows*blockIdx.z: one 8-row tile, or, for unsplit plans, two tiles at once (a 16-row causal window is exactly
 // two consecutive tiles). Queries [kv_head][stride][group][D]; each tile keeps its own partial slot
 // (tile*heads + head)*splits + split of 48 fused rows.
-// kShaped: scores pass a shape (score_shape.cuh) and the CTA walks the list of pages that a row of its window sees.
-template <uint32_t Format, uint32_t Rows, bool kTree, bool kPrefill = false, bool kShaped = false>
+template <uint32_t Format, uint32_t Rows, bool kTree, bool kPrefill = false>
 __global__ void __launch_bounds__(kThreads, 1)
 window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs args) {
   using Kind = Traits<Format>;
@@ -114,30 +111,9 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
   const uint32_t visible = p.committed_tokens + p.active_rows;
   const uint32_t pages = rk_pages_for(visible);
   const uint32_t per_split = rk_pages_per_split(pages, p.split_count);
-  uint32_t page_begin = split * per_split; // shaped: ordinals of the page list, not pages
+  const uint32_t page_begin = split * per_split;
   if (page_begin >= pages) return; // a split without pages writes nothing
-  uint32_t page_end = min(pages, page_begin + per_split);
-  PageList list;
-  if (kShaped) {
-    // The merge counts the splits that exist from the whole context; the listed pages are dealt to that many, in whole
-    // groups. A split that gets none leaves an empty partial.
-    list = PageList::make(p.committed_tokens, visible - 1, 0, args.shape);
-    const uint32_t written = (pages + per_split - 1) / per_split;
-    const uint32_t share = ((list.count + written - 1) / written + 1) & ~1u;
-    page_begin = split * share;
-    page_end = min(list.count, page_begin + share);
-    if (page_begin >= list.count) {
-      constexpr uint32_t kEmptyRows = kPrefill ? RK_PREFILL_TILE_ROWS * kG : kRealRows; // a split prefill plan has one tile per CTA
-      const uint64_t slot = (uint64_t(lane_index) * kHeads + kv_head) * p.slot_splits + split;
-      for (uint32_t i = tid; i < kEmptyRows * kD; i += kThreads) args.partials[slot * kEmptyRows * kD + i] = 0.0f;
-      for (uint32_t i = tid; i < kEmptyRows; i += kThreads) {
-        args.statistics[(slot * kEmptyRows + i) * 2] = -INFINITY;
-        args.statistics[(slot * kEmptyRows + i) * 2 + 1] = 0.0f;
-      }
-      return;
-    }
-  }
-  auto page_of = [&](uint32_t o) { return kShaped ? list.page(o) : o; };
+  const uint32_t page_end = min(pages, page_begin + per_split);
   const uint32_t groups = (page_end - page_begin + 1) / 2;
   const rk_page_entry *table = kPrefill ? args.prefill_table : args.tables[lane_index];
   const uint32_t *row_masks = kTree ? args.row_masks + uint64_t(lane_index) * p.row_capacity : nullptr;
@@ -245,16 +221,16 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
     const uint32_t page_stride = kind < 2 ? data_bytes : scale_bytes, copy_bytes = kind < 2 ? kSlab : 128u;
     auto source = [&](rk_page_entry entry) { return rk_entry_extent(entry) + tensor_base + uint64_t(rk_entry_index(entry)) * page_stride; };
     // table entries travel one group ahead of their use (copies) and of their L2 request (prefetch)
-    rk_page_entry next = lane < 8 && page_begin + local < page_end ? table[page_of(page_begin + local)] : 0;
-    rk_page_entry next_ahead = prefetcher && page_begin + 2 * kPrefetchGroups + local < page_end ? table[page_of(page_begin + 2 * kPrefetchGroups + local)] : 0;
+    rk_page_entry next = lane < 8 && page_begin + local < page_end ? table[page_begin + local] : 0;
+    rk_page_entry next_ahead = prefetcher && page_begin + 2 * kPrefetchGroups + local < page_end ? table[page_begin + 2 * kPrefetchGroups + local] : 0;
     const uint32_t issued = groups - min(groups, args.withheld_groups); // all of them, except under the timeout probe
     for (uint32_t g = 0; g < issued; ++g) {
       const uint32_t r = g % kRawStages;
       const uint32_t first = page_begin + 2 * g, group_pages = min(2u, page_end - first);
       const rk_page_entry entry = next, entry_ahead = next_ahead;
       const uint32_t ahead = first + 2 * kPrefetchGroups + local;
-      if (lane < 8 && first + 2 + local < page_end) next = table[page_of(first + 2 + local)];
-      if (prefetcher && ahead + 2 < page_end) next_ahead = table[page_of(ahead + 2)];
+      if (lane < 8 && first + 2 + local < page_end) next = table[first + 2 + local];
+      if (prefetcher && ahead + 2 < page_end) next_ahead = table[ahead + 2];
       if (g >= kRawStages) barrier_wait(&ctl.raw_free[r], g / kRawStages - 1, error); // the stage's last readers
       const uint32_t full = smem_u32(&ctl.raw_full[r]), stage = raw_tile + r * kRawStageBytes;
       if (lane == 0) barrier_expect(full, group_pages * (2 * kSlab + (Kind::kScales ? 256 : 0)));
@@ -335,16 +311,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
       const uint32_t r = g % kRawStages, slot = r, b = team, round = g / kTileStages;
       const uint32_t first = page_begin + 2 * g;
       // positions of the group whose tokens exist: the split may end inside the group, the lane inside the page
-      const auto valid = [&] {
-        if constexpr (kShaped) {
-          const GroupView view{list.page(first) * kPageTokens, list.page(first + 1) * kPageTokens, first + 1 < page_end};
-          if (view.whole(visible - 1, list.window_first)) return ValidBits{~uint64_t(0)};
-          return ValidBits{uint64_t(view.seen_first(visible - 1, list.window_first, args.shape.sinks)) |
-                           uint64_t(view.seen_second(visible - 1, list.window_first, args.shape.sinks)) << 32};
-        } else {
-          return ValidBelow{min(min(2u, page_end - first) * kPageTokens, visible - first * kPageTokens)};
-        }
-      }();
+      const ValidBelow valid{min(min(2u, page_end - first) * kPageTokens, visible - first * kPageTokens)};
       const uint8_t *raw = raw_ptr + r * kRawStageBytes;
       barrier_wait(&ctl.raw_full[slot], g / kRawStages, error);
       // per-position scale triples {key scale, log2 value scale, 2^-6 / value scale}; zeros past the valid tokens
@@ -385,9 +352,6 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
     const uint32_t query_row = my_row / kG;
     const uint32_t causal_limit = min(visible, p.committed_tokens + min(query_row, p.active_rows - 1) + 1);
     const uint32_t tree_mask = kTree && query_row < p.row_capacity ? row_masks[query_row] : 0u;
-    const uint32_t row_position = p.committed_tokens + min(query_row, p.active_rows - 1);
-    const uint32_t row_window = kShaped && args.shape.window && row_position + 1 > args.shape.window ? row_position + 1 - args.shape.window : 0;
-    const float slope = kShaped && args.shape.slopes && my_row < kRealRows ? __ldg(args.shape.slopes + kv_head * kG + my_row % kG) * kLog2e : 0.0f;
     const uint32_t lane_address = (quarter * 32u) << 16;
     constexpr uint32_t kOutColumns = kD / kRowThreads; // columns of O this thread rescales and writes out
     float row_max = -1.0e30f, row_sum = 0.0f;          // row_sum: this thread's tokens only
@@ -409,14 +373,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
       tmem_load_scores(tmem_s + b * 64 + lane_address + part * kRowTokens, scores);
 
       float group_max = -INFINITY;
-      if constexpr (kShaped) {
-        // the two pages of a group need not be neighbours
-        const GroupView view{list.page(first) * kPageTokens, list.page(first + 1) * kPageTokens, present > kPageTokens};
-        shape_scores<kRowTokens, kPermuted>(scores, stage, part * kRowTokens, row_factor, row_offset, part_token, args.shape, slope, view, row_position);
-        mask_scores<kRowTokens, kPermuted>(scores, part_token, view, row_position, row_window, args.shape.sinks);
-#pragma unroll
-        for (uint32_t i = 0; i < kRowTokens; ++i) group_max = fmaxf(group_max, scores[i]);
-      } else if (!kTree && limit >= kGroupTokens) { // every token of the group is admitted (all but the last groups of a lane)
+      if (!kTree && limit >= kGroupTokens) { // every token of the group is admitted (all but the last groups of a lane)
         scale_scores(scores, stage, part * kRowTokens, row_factor, row_offset);
 #pragma unroll
         for (uint32_t i = 0; i < kRowTokens; ++i) group_max = fmaxf(group_max, scores[i]);
@@ -539,7 +496,7 @@ using namespace rk;
 // rk_attention_verify_reduce.
 namespace {
 template <uint32_t Format>
-int launch_window(const Window *w, uint32_t lanes, uint32_t row_capacity, uint32_t grid_splits, const VerifyArgs &args, bool shaped, cudaStream_t s) {
+int launch_window(const Window *w, uint32_t lanes, uint32_t row_capacity, uint32_t grid_splits, const VerifyArgs &args, cudaStream_t s) {
   constexpr size_t shared_bytes = 1024 + tile_bytes<Format>() + sizeof(Control);
   const CUtensorMap &map = Format == RK_FORMAT_INT4 ? w->int4_head_map : Format == RK_FORMAT_BF16 ? w->int4_map : w->byte_head_map;
   const dim3 grid(kHeads, grid_splits, lanes);
@@ -549,8 +506,6 @@ int launch_window(const Window *w, uint32_t lanes, uint32_t row_capacity, uint32
     return kOk;
   };
   const bool tree = args.row_masks != nullptr;
-  if (shaped) // one row takes the streaming kernels
-    return row_capacity == 8 ? launch(window_attention_kernel<Format, 8, false, false, true>) : launch(window_attention_kernel<Format, 16, false, false, true>);
   if (row_capacity == 1) return launch(window_attention_kernel<Format, 1, false>);
   if (row_capacity == 8) return tree ? launch(window_attention_kernel<Format, 8, true>) : launch(window_attention_kernel<Format, 8, false>);
   return tree ? launch(window_attention_kernel<Format, 16, true>) : launch(window_attention_kernel<Format, 16, false>);
@@ -562,7 +517,7 @@ static int verify_split_tc(const void *window, uint32_t format, uint32_t kv_head
                            const void *queries, float *partials, float *statistics,
                            const rk_page_entry *const *tables, const uint32_t *row_masks,
                            const rk_verify_params *lane_params, rk_kv_layer layer, uint32_t *status,
-                           uint32_t spin_limit, uint32_t withheld_groups, const ShapeArgs *shape, void *stream) {
+                           uint32_t spin_limit, uint32_t withheld_groups, void *stream) {
   if (kv_heads != kHeads || query_heads != kHeads * kG || head_dim != kD || !rk_format_valid(format) ||
       (row_capacity != 1 && row_capacity != 8 && row_capacity != 16) || (row_capacity == 1 && row_masks) ||
       (format == RK_FORMAT_FP8E4M3 && row_masks)) {
@@ -576,14 +531,14 @@ static int verify_split_tc(const void *window, uint32_t format, uint32_t kv_head
     return kInvalid;
   }
   VerifyArgs args{static_cast<const uint16_t *>(queries), partials, statistics, tables, row_masks, lane_params, layer, w->base, status,
-                  spin_limit, withheld_groups, nullptr, {}, shape ? *shape : ShapeArgs{}};
+                  spin_limit, withheld_groups, nullptr, {}};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int st = kUnsupported;
   switch (format) {
-  case RK_FORMAT_INT4: st = launch_window<RK_FORMAT_INT4>(w, lanes, row_capacity, grid_splits, args, shape != nullptr, s); break;
-  case RK_FORMAT_INT8: st = launch_window<RK_FORMAT_INT8>(w, lanes, row_capacity, grid_splits, args, shape != nullptr, s); break;
-  case RK_FORMAT_FP8E4M3: st = launch_window<RK_FORMAT_FP8E4M3>(w, lanes, row_capacity, grid_splits, args, shape != nullptr, s); break;
-  case RK_FORMAT_BF16: st = launch_window<RK_FORMAT_BF16>(w, lanes, row_capacity, grid_splits, args, shape != nullptr, s); break;
+  case RK_FORMAT_INT4: st = launch_window<RK_FORMAT_INT4>(w, lanes, row_capacity, grid_splits, args, s); break;
+  case RK_FORMAT_INT8: st = launch_window<RK_FORMAT_INT8>(w, lanes, row_capacity, grid_splits, args, s); break;
+  case RK_FORMAT_FP8E4M3: st = launch_window<RK_FORMAT_FP8E4M3>(w, lanes, row_capacity, grid_splits, args, s); break;
+  case RK_FORMAT_BF16: st = launch_window<RK_FORMAT_BF16>(w, lanes, row_capacity, grid_splits, args, s); break;
   }
   if (st) return st;
   return cuda_status(cudaGetLastError(), "window kernel launch");
@@ -596,27 +551,7 @@ extern "C" int rk_attention_verify_split_tc(const void *window, uint32_t format,
                                             const rk_verify_params *lane_params, rk_kv_layer layer, uint32_t *status,
                                             void *stream) {
   return verify_split_tc(window, format, kv_heads, query_heads, head_dim, lanes, row_capacity, grid_splits, queries, partials,
-                         statistics, tables, row_masks, lane_params, layer, status, kSpinLimit, 0, nullptr, stream);
-}
-
-// rk_attention_verify_split_tc with a score shape: chain windows of 8 or 16 rows, every format. Only the pages that a row
-// of the window sees are read.
-extern "C" int rk_attention_verify_split_shaped(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,
-                                                uint32_t head_dim, uint32_t lanes, uint32_t row_capacity, uint32_t grid_splits,
-                                                const void *queries, float *partials, float *statistics,
-                                                const rk_page_entry *const *tables, const rk_verify_params *lane_params,
-                                                rk_kv_layer layer, const rk_score_shape *shape, uint32_t *status, void *stream) {
-  ShapeArgs shape_args;
-  if (row_capacity == 1) {
-    set_error("rk_attention_verify_split_shaped: row capacity 8 or 16; one row takes rk_attention_decode_shaped");
-    return kUnsupported;
-  }
-  if (!shape || !shape_arguments(shape, shape_args)) {
-    set_error("rk_attention_verify_split_shaped: invalid shape");
-    return kInvalid;
-  }
-  return verify_split_tc(window, format, kv_heads, query_heads, head_dim, lanes, row_capacity, grid_splits, queries, partials,
-                         statistics, tables, nullptr, lane_params, layer, status, kSpinLimit, 0, &shape_args, stream);
+                         statistics, tables, row_masks, lane_params, layer, status, kSpinLimit, 0, stream);
 }
 
 // Test hook of the window kernel's timeout path: the same launch with waits that give up after `spin_limit` polls
@@ -631,15 +566,16 @@ extern "C" int rk_attention_verify_probe_timeout(const void *window, uint32_t fo
                                                  uint32_t withheld_groups, void *stream) {
   if (!spin_limit || spin_limit > kSpinLimit) { set_error("rk_attention_verify_probe_timeout: spin limit out of range"); return kInvalid; }
   return verify_split_tc(window, format, kv_heads, query_heads, head_dim, lanes, row_capacity, grid_splits, queries, partials,
-                         statistics, tables, nullptr, lane_params, layer, status, spin_limit, withheld_groups, nullptr, stream);
+                         statistics, tables, nullptr, lane_params, layer, status, spin_limit, withheld_groups, stream);
 }
 
 // prefill_attention_*_split (prefill/paged_attention.metal:7-67) on the tcgen05 kernel: one CTA per (KV head, split,
 // 8-row tile). Arguments and scratch layout as rk_attention_prefill_split plus the pool's window and the status
 // word; merge with rk_attention_prefill_reduce. `params` is a HOST pointer.
-static int prefill_split_tc(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads, uint32_t head_dim,
-                            const void *queries, float *partials, float *statistics, const rk_page_entry *table,
-                            const rk_prefill_params *params, uint32_t *status, const ShapeArgs *shape, void *stream) {
+extern "C" int rk_attention_prefill_split_tc(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,
+                                             uint32_t head_dim, const void *queries, float *partials, float *statistics,
+                                             const rk_page_entry *table, const rk_prefill_params *params, uint32_t *status,
+                                             void *stream) {
   if (kv_heads != kHeads || query_heads != kHeads * kG || head_dim != kD || !rk_format_valid(format)) {
     set_error("rk_attention_prefill_split_tc: built for 4 KV heads x 24 query heads x 256");
     return kUnsupported;
@@ -650,7 +586,7 @@ static int prefill_split_tc(const void *window, uint32_t format, uint32_t kv_hea
     return kInvalid;
   }
   VerifyArgs args{static_cast<const uint16_t *>(queries), partials, statistics, nullptr, nullptr, nullptr, params->kv, w->base, status,
-                  kSpinLimit, 0, table, *params, shape ? *shape : ShapeArgs{}};
+                  kSpinLimit, 0, table, *params};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const uint32_t tiles = (params->rows + RK_PREFILL_TILE_ROWS - 1) / RK_PREFILL_TILE_ROWS;
   const bool pairs = params->split_count == 1 && tiles > 1; // two tiles per CTA fill 96 of the 128 tensor-core rows
@@ -663,9 +599,6 @@ static int prefill_split_tc(const void *window, uint32_t format, uint32_t kv_hea
   auto launch_format = [&](auto format_tag, const CUtensorMap &map) -> int {
     constexpr uint32_t F = decltype(format_tag)::value;
     constexpr size_t shared_bytes = 1024 + tile_bytes<F>() + sizeof(Control);
-    if (shape)
-      return pairs ? launch(window_attention_kernel<F, 16, false, true, true>, shared_bytes, map)
-                   : launch(window_attention_kernel<F, 8, false, true, true>, shared_bytes, map);
     return pairs ? launch(window_attention_kernel<F, 16, false, true>, shared_bytes, map)
                  : launch(window_attention_kernel<F, 8, false, true>, shared_bytes, map);
   };
@@ -675,24 +608,4 @@ static int prefill_split_tc(const void *window, uint32_t format, uint32_t kv_hea
   case RK_FORMAT_FP8E4M3: return launch_format(std::integral_constant<uint32_t, RK_FORMAT_FP8E4M3>{}, w->byte_head_map);
   default: return launch_format(std::integral_constant<uint32_t, RK_FORMAT_BF16>{}, w->int4_map);
   }
-}
-
-extern "C" int rk_attention_prefill_split_tc(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,
-                                             uint32_t head_dim, const void *queries, float *partials, float *statistics,
-                                             const rk_page_entry *table, const rk_prefill_params *params, uint32_t *status,
-                                             void *stream) {
-  return prefill_split_tc(window, format, kv_heads, query_heads, head_dim, queries, partials, statistics, table, params, status, nullptr, stream);
-}
-
-// The same with a score shape.
-extern "C" int rk_attention_prefill_split_shaped(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,
-                                                 uint32_t head_dim, const void *queries, float *partials, float *statistics,
-                                                 const rk_page_entry *table, const rk_prefill_params *params,
-                                                 const rk_score_shape *shape, uint32_t *status, void *stream) {
-  ShapeArgs shape_args;
-  if (!shape || !shape_arguments(shape, shape_args)) {
-    set_error("rk_attention_prefill_split_shaped: invalid shape");
-    return kInvalid;
-  }
-  return prefill_split_tc(window, format, kv_heads, query_heads, head_dim, queries, partials, statistics, table, params, status, &shape_args, stream);
 }

@@ -215,6 +215,12 @@ __device__ __forceinline__ void tmem_store8(uint32_t address, const uint32_t (&v
                ::"r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_store16(uint32_t address, const float (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+               ::"r"(address), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]),
+                 "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]) : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void tmem_load_scores(uint32_t address, float (&v)[16]) { tmem_load16(address, v); }
 __device__ __forceinline__ void tmem_store_packed(uint32_t address, const uint32_t (&v)[8]) { tmem_store8(address, v); }
 __device__ __forceinline__ float exp2_fast(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
@@ -493,57 +499,5 @@ struct GroupView {
     return both ? seen_tokens(second, position, window_first, sinks) : 0u;
   }
 };
-
-// Scores of unseen tokens become -infinity. A warp's rows usually see the whole group: nothing is worked out or tested then
-// (the bits cost about as many instructions as the scores of a thread).
-template <uint32_t N, bool kPermuted>
-__device__ __forceinline__ void mask_scores(float (&scores)[N], uint32_t part_token, const GroupView &view, uint32_t position,
-                                            uint32_t window_first, uint32_t sinks, bool real = true) {
-  if (__all_sync(0xffffffffu, !real || view.whole(position, window_first))) return;
-  const uint32_t seen_first = view.seen_first(position, window_first, sinks), seen_second = view.seen_second(position, window_first, sinks);
-  static_assert(kPermuted || N <= kPageTokens, "an unpermuted part lies in one page");
-  const uint32_t mine = part_token < kPageTokens ? seen_first : seen_second;
-#pragma unroll
-  for (uint32_t i = 0; i < N; ++i) {
-    const uint32_t bits = kPermuted ? (local_token<kPermuted>(i) < kPageTokens ? seen_first : seen_second) : mine;
-    if (!((bits >> ((local_token<kPermuted>(i) + part_token) & 31u)) & 1u)) scores[i] = -INFINITY;
-  }
-}
-
-// Accumulators to scores + log2(value scale) through a shape, without the mask. Each stage is one branch for the launch.
-template <uint32_t N, bool kPermuted>
-__device__ __forceinline__ void shape_scores(float (&scores)[N], const ScaleStage &stage, uint32_t first_position, float row_factor,
-                                             float row_offset, uint32_t part_token, const ShapeArgs &shape, float slope,
-                                             const GroupView &view, uint32_t position) {
-  if (shape.cap == 0.0f && !shape.slopes) {
-    scale_scores(scores, stage, first_position, row_factor, row_offset);
-    return;
-  }
-  const float2 factor = make_float2(row_factor, row_factor), offset = make_float2(row_offset, row_offset);
-#pragma unroll
-  for (uint32_t i = 0; i < N; i += 2) {
-    const float2 keys = *reinterpret_cast<const float2 *>(&stage.pairs[(first_position + i) >> 1]);
-    const float2 s = mul_pair(fma_pair(make_float2(scores[i], scores[i + 1]), factor, offset), keys);
-    scores[i] = s.x;
-    scores[i + 1] = s.y;
-  }
-  if (shape.cap > 0.0f) soft_cap(scores, shape.cap, shape.cap_inverse);
-  if (shape.slopes) {
-    const float first = float(int32_t(view.first - position + part_token)), second = float(int32_t(view.second - position + part_token - kPageTokens));
-    const float mine = part_token < kPageTokens ? first : second;
-#pragma unroll
-    for (uint32_t i = 0; i < N; ++i) {
-      const float origin = kPermuted ? (local_token<kPermuted>(i) < kPageTokens ? first : second) : mine;
-      scores[i] = fmaf(slope, origin + float(local_token<kPermuted>(i)), scores[i]);
-    }
-  }
-#pragma unroll
-  for (uint32_t i = 0; i < N; i += 2) {
-    const float2 logs = *(reinterpret_cast<const float2 *>(&stage.pairs[(first_position + i) >> 1]) + 1);
-    const float2 s = add_pair(make_float2(scores[i], scores[i + 1]), logs);
-    scores[i] = s.x;
-    scores[i + 1] = s.y;
-  }
-}
 
 } // namespace rk::tile
