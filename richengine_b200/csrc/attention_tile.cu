@@ -319,6 +319,111 @@ prefill_reduce_kernel(const float *__restrict__ partials, const float *__restric
                       (uint64_t(tile) * KvHeads + kv_head) * p.split_count, fused_row);
 }
 
+// ---- the merge without an epilogue ----------------------------------------------------------------------------------------
+// The same operations in the same order as reduce_row, with four dims a thread and twelve rows a block: a thread takes three
+// rows whose loads are in flight together, and nothing crosses a block barrier. Bound by memory: the partials are read once
+// and the rows written once. (A block of 256 threads per row, one value each, left most of its time between the loads of a
+// row: a 2 048-row chunk's merge took 110 us for 75 MB.)
+constexpr uint32_t kMergeThreads = 256, kMergeRowsPerThread = 3, kMergeRows = kMergeThreads / 64 * kMergeRowsPerThread;
+struct MergeRows {
+  const float *partials, *statistics;
+  uint16_t *output;     // of the tile: [fused row][256]
+  float *output_f32;    // may be null
+  uint32_t committed, active_rows, group, rows, splits; // rows: fused rows of a slot
+  uint64_t head_slot;
+};
+__device__ __forceinline__ void store_quad(const MergeRows &m, uint32_t row, uint32_t quad, float4 value) {
+  const uint32_t low = uint32_t(float_to_bf16_bits(value.x)) | uint32_t(float_to_bf16_bits(value.y)) << 16;
+  const uint32_t high = uint32_t(float_to_bf16_bits(value.z)) | uint32_t(float_to_bf16_bits(value.w)) << 16;
+  *reinterpret_cast<uint2 *>(m.output + row * 256u + 4 * quad) = make_uint2(low, high);
+  if (m.output_f32) *reinterpret_cast<float4 *>(m.output_f32 + row * 256u + 4 * quad) = value;
+}
+__device__ __forceinline__ void merge_rows(const MergeRows &m, uint32_t block_row) {
+  const uint32_t quad = threadIdx.x & 63u, lane = threadIdx.x % 32, first = block_row + threadIdx.x / 64;
+  constexpr uint32_t kStep = kMergeThreads / 64;
+  const uint32_t live = min(m.rows, m.active_rows * m.group);
+  const uint32_t pages = rk_pages_for(m.committed + m.active_rows), per_split = rk_pages_per_split(pages, m.splits);
+  const uint32_t written = (pages + per_split - 1) / per_split;
+  auto stat_of = [&](uint32_t s, uint32_t row) { return reinterpret_cast<const float2 *>(m.statistics) + ((m.head_slot + s) * m.rows + row); };
+  auto part_of = [&](uint32_t s, uint32_t row) { return reinterpret_cast<const float4 *>(m.partials) + ((m.head_slot + s) * m.rows + row) * 64 + quad; };
+  auto quotient = [](float4 n, float d) {
+    return d > 0.0f ? make_float4(n.x / d, n.y / d, n.z / d, n.w / d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  };
+  if (written == 1) { // the weight is exp(0)
+    float2 stat[kMergeRowsPerThread];
+    float4 part[kMergeRowsPerThread];
+#pragma unroll
+    for (uint32_t r = 0; r < kMergeRowsPerThread; ++r) {
+      const uint32_t row = first + r * kStep;
+      if (row < live) { stat[r] = __ldg(stat_of(0, row)); part[r] = __ldg(part_of(0, row)); }
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < kMergeRowsPerThread; ++r) {
+      const uint32_t row = first + r * kStep;
+      if (row >= m.rows) continue;
+      const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f); // added as the sum does: -0 becomes 0
+      store_quad(m, row, quad, row < live ? quotient(make_float4(zero.x + part[r].x, zero.y + part[r].y, zero.z + part[r].z, zero.w + part[r].w), stat[r].y) : zero);
+    }
+    return;
+  }
+  for (uint32_t r = 0; r < kMergeRowsPerThread; ++r) {
+    const uint32_t row = first + r * kStep; // the same for a whole warp
+    if (row >= m.rows) break;
+    float4 numerator = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float denominator = 0.0f;
+    if (row < live) {
+      float maximum = -INFINITY;
+      for (uint32_t s = lane; s < written; s += 32) maximum = fmaxf(maximum, __ldg(stat_of(s, row)).x);
+      maximum = warp_max(maximum);
+      constexpr uint32_t kBatch = 4;
+      for (uint32_t base = 0; base < written; base += kBatch) { // in split order
+        float2 stat[kBatch];
+        float4 part[kBatch];
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k)
+          if (base + k < written) { stat[k] = __ldg(stat_of(base + k, row)); part[k] = __ldg(part_of(base + k, row)); }
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k)
+          if (base + k < written) {
+            const float weight = expf(stat[k].x - maximum);
+            numerator.x += weight * part[k].x; numerator.y += weight * part[k].y;
+            numerator.z += weight * part[k].z; numerator.w += weight * part[k].w;
+            denominator += weight * stat[k].y;
+          }
+      }
+    }
+    store_quad(m, row, quad, quotient(numerator, denominator));
+  }
+}
+
+// grid (blocks of rows, kv_heads, lanes)
+template <uint32_t KvHeads>
+__global__ void __launch_bounds__(kMergeThreads, 4)
+verify_merge_kernel(const float *__restrict__ partials, const float *__restrict__ statistics, uint16_t *__restrict__ output,
+                    float *__restrict__ output_f32, const rk_verify_params *__restrict__ lane_params, uint32_t group) {
+  const uint32_t kv_head = blockIdx.y, lane_index = blockIdx.z, block_row = blockIdx.x * kMergeRows;
+  rk_verify_params p = lane_params[lane_index];
+  p.kv.extent_pages = 1; // placement plays no part in the merge
+  if (!rk_verify_contract_valid(&p) || block_row >= p.row_capacity * group) return;
+  const uint64_t tile = (uint64_t(lane_index) * KvHeads + kv_head) * (uint64_t(RK_VERIFY_CHUNK_STRIDE) * group * 256);
+  merge_rows({partials, statistics, output + tile, output_f32 ? output_f32 + tile : nullptr, p.committed_tokens, p.active_rows, group,
+              p.row_capacity * group, p.split_count, (uint64_t(lane_index) * KvHeads + kv_head) * p.slot_splits}, block_row);
+}
+
+// grid (blocks of rows, kv_heads, tiles)
+template <uint32_t KvHeads>
+__global__ void __launch_bounds__(kMergeThreads, 4)
+prefill_merge_kernel(const float *__restrict__ partials, const float *__restrict__ statistics, uint16_t *__restrict__ output,
+                     float *__restrict__ output_f32, rk_prefill_params p, uint32_t group) {
+  const uint32_t kv_head = blockIdx.y, tile = blockIdx.z, tile_start = tile * RK_PREFILL_TILE_ROWS, block_row = blockIdx.x * kMergeRows;
+  p.kv.extent_pages = 1;
+  if (!rk_prefill_contract_valid(&p) || tile_start >= p.rows) return;
+  const uint64_t offset = (uint64_t(kv_head) * p.chunk_stride + tile_start) * group * 256;
+  merge_rows({partials, statistics, output + offset, output_f32 ? output_f32 + offset : nullptr, p.committed_tokens + tile_start,
+              min(RK_PREFILL_TILE_ROWS, p.rows - tile_start), group, RK_PREFILL_TILE_ROWS * group, p.split_count,
+              (uint64_t(tile) * KvHeads + kv_head) * p.split_count}, block_row);
+}
+
 template <typename Kernel> int allow_shared(Kernel kernel, size_t bytes) {
   return cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)),
                      "cudaFuncSetAttribute(shared memory)");
@@ -362,6 +467,12 @@ int launch_prefill_split(const void *queries, float *partials, float *statistics
   kernel<<<dim3(4, tiles, p.split_count), kThreads, bytes, stream>>>(
       static_cast<const uint16_t *>(queries), partials, statistics, table, p);
   return cuda_status(cudaGetLastError(), "prefill split launch");
+}
+
+// Whether the wide merge may load and store these; others take the merge of one value per thread.
+bool quad_aligned(const void *partials, const void *statistics, const void *output, const void *output_f32) {
+  return !((reinterpret_cast<uintptr_t>(partials) | reinterpret_cast<uintptr_t>(output_f32)) & 15u) &&
+         !((reinterpret_cast<uintptr_t>(statistics) | reinterpret_cast<uintptr_t>(output)) & 7u);
 }
 
 bool supported_geometry(uint32_t kv_heads, uint32_t query_heads, uint32_t head_dim) {
@@ -412,8 +523,12 @@ extern "C" int rk_attention_verify_reduce(uint32_t kv_heads, uint32_t query_head
     return kInvalid;
   }
   const uint32_t group = query_heads / kv_heads;
-  verify_reduce_kernel<4, 256><<<dim3(kv_heads, row_capacity * group, lanes), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      partials, statistics, static_cast<uint16_t *>(output), output_f32, lane_params, group, nullptr, nullptr);
+  if (!quad_aligned(partials, statistics, output, output_f32))
+    verify_reduce_kernel<4, 256><<<dim3(kv_heads, row_capacity * group, lanes), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        partials, statistics, static_cast<uint16_t *>(output), output_f32, lane_params, group, nullptr, nullptr);
+  else
+    verify_merge_kernel<4><<<dim3((row_capacity * group + kMergeRows - 1) / kMergeRows, kv_heads, lanes), kMergeThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+      partials, statistics, static_cast<uint16_t *>(output), output_f32, lane_params, group);
   return cuda_status(cudaGetLastError(), "verify reduce launch");
 }
 
@@ -468,7 +583,11 @@ extern "C" int rk_attention_prefill_reduce(uint32_t kv_heads, uint32_t query_hea
   }
   const uint32_t group = query_heads / kv_heads;
   const uint32_t tiles = (params->rows + RK_PREFILL_TILE_ROWS - 1) / RK_PREFILL_TILE_ROWS;
-  prefill_reduce_kernel<4, 256><<<dim3(kv_heads, RK_PREFILL_TILE_ROWS * group, tiles), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+  if (!quad_aligned(partials, statistics, output, output_f32))
+    prefill_reduce_kernel<4, 256><<<dim3(kv_heads, RK_PREFILL_TILE_ROWS * group, tiles), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        partials, statistics, static_cast<uint16_t *>(output), output_f32, *params, group);
+  else
+    prefill_merge_kernel<4><<<dim3(RK_PREFILL_TILE_ROWS * group / kMergeRows, kv_heads, tiles), kMergeThreads, 0, static_cast<cudaStream_t>(stream)>>>(
       partials, statistics, static_cast<uint16_t *>(output), output_f32, *params, group);
   return cuda_status(cudaGetLastError(), "prefill reduce launch");
 }
