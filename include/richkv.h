@@ -298,11 +298,9 @@ int rk_session_status(void *session, void *stream);
  * may have, more pages than it names or the table holds, or names a page past page_count is made idle (no live rows: every
  * kernel skips it; its slots are all ones) and raises the sticky `status` word. Every page named has to lie in an extent
  * that the pool holds. At most 1 024 lanes; row_slots takes lanes * row_capacity words. */
-int rk_step_tables(const rk_step_pool *pool, uint32_t lanes, uint32_t table_pages, uint32_t row_capacity,
-                   uint32_t split_count, float score_scale, const uint32_t *page_ids, const uint32_t *page_offsets,
+int rk_step_tables(const rk_step_layout *layout, const uint32_t *page_ids, const uint32_t *page_offsets,
                    const uint32_t *committed, const uint32_t *rows, const uint32_t *known_pages,
-                   rk_page_entry *entries, rk_chunk_params *chunk_params, rk_verify_params *verify_params,
-                   uint32_t *row_offsets, uint64_t *row_slots, uint32_t *status, void *stream);
+                   const rk_step_outputs *outputs, void *stream);
 /* Which lanes share how long a prefix, from their tables (equal entries are the same page; only pages full on every side
  * count). Lanes are gathered under the lowest lane that has their first page; of those, the ones that share the p pages
  * for which (lanes - 1) * p is largest (ties: the larger p) become a group, if there are at least minimum_lanes (>= 2) of

@@ -114,6 +114,25 @@ typedef struct rk_step_pool {
   uint32_t extent_pages, page_count;
 } rk_step_pool;
 
+/* What a batch's step tables look like (rk_step_tables): the same from step to step. */
+typedef struct rk_step_layout {
+  rk_step_pool pool;
+  uint32_t lanes, table_pages, row_capacity, split_count;
+  float score_scale;
+  uint32_t reserved; /* 0 */
+} rk_step_layout;
+
+/* Where they go (device memory): entries [lane][table_pages], one parameter block of each kind per lane, row_offsets
+ * [lanes + 1], row_slots [lanes * row_capacity], one status word. */
+typedef struct rk_step_outputs {
+  rk_page_entry *entries;
+  rk_chunk_params *chunk_params;
+  rk_verify_params *verify_params;
+  uint32_t *row_offsets;
+  uint64_t *row_slots;
+  uint32_t *status;
+} rk_step_outputs;
+
 /* A lane that belongs to no group of lanes with a shared prefix. */
 #define RK_NO_GROUP 0xffffffffu
 
@@ -130,7 +149,7 @@ static_assert(sizeof(rk_prefill_params) == 32, "prefill parameters are 32 bytes"
 static_assert(sizeof(rk_verify_params) == 36, "verify parameters are 36 bytes");
 static_assert(sizeof(rk_page_copy) == 8, "page copy is 8 bytes");
 static_assert(sizeof(rk_score_shape) == 24 && offsetof(rk_score_shape, slopes) == 16, "score shape is 24 bytes");
-static_assert(sizeof(rk_step_pool) == 24, "step pool is 24 bytes");
+static_assert(sizeof(rk_step_pool) == 24 && sizeof(rk_step_layout) == 48 && sizeof(rk_step_outputs) == 48, "step table blocks");
 static_assert(offsetof(rk_chunk_params, kv) == 16, "chunk kv offset");
 static_assert(offsetof(rk_prefill_params, kv) == 16 &&
                   offsetof(rk_prefill_params, split_count) == 24 &&

@@ -11,20 +11,13 @@ namespace rk {
 namespace {
 
 constexpr uint32_t kMaxLanes = 1024;
-constexpr uint32_t kTableThreads = 512;
+constexpr uint32_t kTableThreads = 256;
 constexpr uint32_t kGroupThreads = 256;
 
 struct StepArgs {
   const uint32_t *page_ids, *page_offsets, *committed, *rows, *known_pages;
-  uint64_t base, extent_stride;
-  uint32_t extent_pages, page_count, lanes, table_pages, row_capacity, split_count;
-  float score_scale;
-  rk_page_entry *entries;
-  rk_chunk_params *chunk_params;
-  rk_verify_params *verify_params;
-  uint32_t *row_offsets;
-  uint64_t *row_slots;
-  uint32_t *status;
+  rk_step_layout layout;
+  rk_step_outputs out;
 };
 
 __device__ __forceinline__ uint32_t block_sum(uint32_t value, uint32_t *scratch) {
@@ -41,46 +34,57 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t value, uint32_t *scratch)
 
 // One block per lane: the lane is refused as a whole (its parameter blocks say so), so one block has to see all of its
 // page ids before it writes them. Bound by memory where tables are built anew (4 bytes in, 8 out per page), by latency
-// where only the pages behind `known_pages` are.
+// where only the pages behind `known_pages` are. 256 threads: eight blocks of an SM hold the largest batch in one wave.
 __global__ void __launch_bounds__(kTableThreads)
-step_tables_kernel(StepArgs a) {
+step_tables_kernel(const __grid_constant__ StepArgs a) {
   __shared__ uint32_t scratch[kTableThreads / 32];
-  const uint32_t l = blockIdx.x, tid = threadIdx.x;
-  uint32_t before = 0; // rows of the lanes before this one
-  for (uint32_t i = tid; i < l; i += kTableThreads) before += min(a.rows[i], a.row_capacity);
+  const uint32_t l = blockIdx.x, tid = threadIdx.x, capacity = a.layout.row_capacity, page_count = a.layout.pool.page_count;
   const uint32_t begin = a.page_offsets[l], end = a.page_offsets[l + 1], committed = a.committed[l], rows = a.rows[l];
+  const uint32_t known = a.known_pages ? a.known_pages[l] : 0;
+  uint32_t before = 0; // rows of the lanes before this one
+  for (uint32_t i = tid; i < l; i += kTableThreads) before += min(a.rows[i], capacity);
   const uint32_t count = end >= begin ? end - begin : 0;
   const uint64_t tokens = uint64_t(committed) + rows;
-  bool good = rows > 0 && rows <= a.row_capacity && end >= begin && tokens <= RK_MAX_PHYSICAL_TOKENS &&
-              rk_pages_for(uint32_t(tokens)) <= min(count, a.table_pages);
+  bool good = rows > 0 && rows <= capacity && end >= begin && tokens <= RK_MAX_PHYSICAL_TOKENS &&
+              rk_pages_for(uint32_t(tokens)) <= min(count, a.layout.table_pages);
   const uint32_t pages = good ? rk_pages_for(uint32_t(tokens)) : 0;
-  const uint32_t first = a.known_pages ? min(a.known_pages[l], pages) : 0;
   const uint32_t *ids = a.page_ids + begin;
-  rk_page_entry *table = a.entries + uint64_t(l) * a.table_pages;
-  for (uint32_t j = first + tid; j < pages; j += kTableThreads) {
-    const uint32_t id = ids[j];
-    if (id >= a.page_count) { good = false; continue; }
-    const uint32_t extent = id / a.extent_pages;
-    table[j] = rk_make_entry(a.base + extent * a.extent_stride, id - extent * a.extent_pages);
+  rk_page_entry *table = a.out.entries + uint64_t(l) * a.layout.table_pages;
+  constexpr uint32_t kBatch = 8; // ids of a thread in flight
+  for (uint32_t base = min(known, pages); base < pages; base += kTableThreads * kBatch) {
+    uint32_t id[kBatch];
+#pragma unroll
+    for (uint32_t k = 0; k < kBatch; ++k) {
+      const uint32_t j = base + k * kTableThreads + tid;
+      id[k] = j < pages ? __ldg(ids + j) : 0;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kBatch; ++k) {
+      const uint32_t j = base + k * kTableThreads + tid;
+      if (j >= pages) break;
+      if (id[k] >= page_count) { good = false; continue; }
+      const uint32_t extent = id[k] / a.layout.pool.extent_pages;
+      table[j] = rk_make_entry(a.layout.pool.base + extent * a.layout.pool.extent_stride, id[k] - extent * a.layout.pool.extent_pages);
+    }
   }
   // the new rows' slots; a page among the known ones is looked at here too
-  const uint32_t mine = min(rows, a.row_capacity);
+  const uint32_t mine = min(rows, capacity);
   uint64_t slot = ~uint64_t(0);
   if (tid < mine && pages) {
     const uint32_t position = committed + tid, id = ids[position / kPageTokens];
-    if (id >= a.page_count) good = false;
+    if (id >= page_count) good = false;
     slot = uint64_t(id) * kPageTokens + position % kPageTokens;
   }
   good = !__syncthreads_or(!good);
   before = block_sum(before, scratch);
-  if (tid < mine) a.row_slots[before + tid] = good ? slot : ~uint64_t(0);
+  if (tid < mine) a.out.row_slots[before + tid] = good ? slot : ~uint64_t(0);
   if (tid == 0) {
     const uint32_t live = good ? rows : 0; // a lane without live rows is skipped by every kernel
-    a.row_offsets[l] = before;
-    if (l + 1 == a.lanes) a.row_offsets[a.lanes] = before + mine;
-    a.chunk_params[l] = rk_chunk_params{committed, live, RK_VERIFY_CHUNK_STRIDE, count, rk_kv_layer{0, 0}};
-    a.verify_params[l] = rk_verify_params{committed, count, rk_kv_layer{0, 0}, a.split_count, a.split_count, live, a.row_capacity, a.score_scale};
-    if (!good && rows) atomicOr(a.status, 1u); // rows == 0 is an idle lane
+    a.out.row_offsets[l] = before;
+    if (l + 1 == a.layout.lanes) a.out.row_offsets[l + 1] = before + mine;
+    a.out.chunk_params[l] = rk_chunk_params{committed, live, RK_VERIFY_CHUNK_STRIDE, count, rk_kv_layer{0, 0}};
+    a.out.verify_params[l] = rk_verify_params{committed, count, rk_kv_layer{0, 0}, a.layout.split_count, a.layout.split_count, live, capacity, a.layout.score_scale};
+    if (!good && rows) atomicOr(a.out.status, 1u); // rows == 0 is an idle lane
   }
 }
 
@@ -112,8 +116,19 @@ common_prefix_kernel(uint32_t lanes, const rk_page_entry *const *__restrict__ ta
   if (tid == 0) { found = l; differ = RK_NO_GROUP; }
   __syncthreads();
   const rk_page_entry first = table[0];
-  for (uint32_t i = tid; i < l; i += kGroupThreads)
-    if (full_pages(lane_params[i]) && tables[i][0] == first) { atomicMin(&found, i); break; } // this thread's lowest
+  constexpr uint32_t kRounds = kMaxLanes / kGroupThreads; // every lane's pointer, then every first entry, in flight at once
+  const rk_page_entry *theirs_at[kRounds];
+#pragma unroll
+  for (uint32_t r = 0; r < kRounds; ++r) {
+    const uint32_t i = tid + r * kGroupThreads;
+    theirs_at[r] = i < l && full_pages(lane_params[i]) ? tables[i] : nullptr;
+  }
+  bool same[kRounds];
+#pragma unroll
+  for (uint32_t r = 0; r < kRounds; ++r) same[r] = theirs_at[r] && *theirs_at[r] == first;
+#pragma unroll
+  for (uint32_t r = 0; r < kRounds; ++r)
+    if (same[r]) { atomicMin(&found, tid + r * kGroupThreads); break; } // this thread's lowest
   __syncthreads();
   const uint32_t leader = found;
   uint32_t common = full;
@@ -154,15 +169,24 @@ form_groups_kernel(uint32_t lanes, uint32_t size, uint32_t minimum_lanes, uint32
   const uint32_t leader = tid < lanes ? __ldcg(lane_groups + tid) : RK_NO_GROUP, common = tid < lanes ? __ldcg(group_pages + tid) : 0;
   keys[tid] = leader == RK_NO_GROUP ? 0xffffffffu : leader << 16 | (0xffffu - common);
   best[tid] = 0;
+  // bitonic sort; steps between lanes of a warp need neither shared memory nor a barrier
+  uint32_t held = keys[tid];
   for (uint32_t k = 2; k <= size; k <<= 1)
     for (uint32_t j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
-      const uint32_t other = tid ^ j;
-      if (other > tid) {
-        const uint32_t mine = keys[tid], theirs = keys[other];
-        if ((mine > theirs) == ((tid & k) == 0)) { keys[tid] = theirs; keys[other] = mine; }
+      uint32_t theirs;
+      if (j >= 32) {
+        __syncthreads();
+        keys[tid] = held;
+        __syncthreads();
+        theirs = keys[tid ^ j];
+      } else {
+        theirs = __shfl_xor_sync(0xffffffffu, held, j);
       }
+      const bool low = (tid & j) == 0, ascending = (tid & k) == 0;
+      held = low == ascending ? min(held, theirs) : max(held, theirs);
     }
+  __syncthreads();
+  keys[tid] = held;
   __syncthreads();
   const uint32_t key = keys[tid];
   const bool live = key != 0xffffffffu;
@@ -189,28 +213,26 @@ using namespace rk;
 
 extern "C" {
 
-int rk_step_tables(const rk_step_pool *pool, uint32_t lanes, uint32_t table_pages, uint32_t row_capacity, uint32_t split_count,
-                   float score_scale, const uint32_t *page_ids, const uint32_t *page_offsets, const uint32_t *committed,
-                   const uint32_t *rows, const uint32_t *known_pages, rk_page_entry *entries, rk_chunk_params *chunk_params,
-                   rk_verify_params *verify_params, uint32_t *row_offsets, uint64_t *row_slots, uint32_t *status, void *stream) {
-  if (!lanes || lanes > kMaxLanes || !table_pages || !row_capacity || row_capacity > RK_TREE_NODES || !split_count ||
-      split_count > RK_VERIFY_MAX_SPLITS) {
+int rk_step_tables(const rk_step_layout *layout, const uint32_t *page_ids, const uint32_t *page_offsets, const uint32_t *committed,
+                   const uint32_t *rows, const uint32_t *known_pages, const rk_step_outputs *outputs, void *stream) {
+  if (!layout || !layout->lanes || layout->lanes > kMaxLanes || !layout->table_pages || !layout->row_capacity ||
+      layout->row_capacity > RK_TREE_NODES || !layout->split_count || layout->split_count > RK_VERIFY_MAX_SPLITS) {
     set_error("rk_step_tables: 1..1024 lanes, a row capacity of 1..16, 1..128 splits and at least one table page");
     return kInvalid;
   }
-  if (!pool || !pool->base || (pool->base & RK_PAGE_INDEX_MASK) || !pool->extent_stride || (pool->extent_stride & RK_PAGE_INDEX_MASK) ||
-      !pool->extent_pages || pool->extent_pages > RK_PAGE_INDEX_MASK + 1 || !pool->page_count) {
+  const rk_step_pool &pool = layout->pool;
+  if (!pool.base || (pool.base & RK_PAGE_INDEX_MASK) || !pool.extent_stride || (pool.extent_stride & RK_PAGE_INDEX_MASK) ||
+      !pool.extent_pages || pool.extent_pages > RK_PAGE_INDEX_MASK + 1 || !pool.page_count) {
     set_error("rk_step_tables: extents are 16 KiB-aligned and hold at most 16 384 pages");
     return kInvalid;
   }
-  if (!page_ids || !page_offsets || !committed || !rows || !entries || !chunk_params || !verify_params || !row_offsets || !row_slots || !status) {
+  if (!page_ids || !page_offsets || !committed || !rows || !outputs || !outputs->entries || !outputs->chunk_params || !outputs->verify_params ||
+      !outputs->row_offsets || !outputs->row_slots || !outputs->status) {
     set_error("rk_step_tables: invalid arguments");
     return kInvalid;
   }
-  const StepArgs args{page_ids, page_offsets, committed, rows, known_pages, pool->base, pool->extent_stride, pool->extent_pages, pool->page_count,
-                      lanes, table_pages, row_capacity, split_count, score_scale, entries, chunk_params, verify_params, row_offsets,
-                      row_slots, status};
-  step_tables_kernel<<<lanes, kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(args);
+  step_tables_kernel<<<layout->lanes, kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+      StepArgs{page_ids, page_offsets, committed, rows, known_pages, *layout, *outputs});
   return cuda_status(cudaGetLastError(), "step tables launch");
 }
 

@@ -57,6 +57,18 @@ class StepPool(C.Structure):
     _fields_ = [("base", C.c_uint64), ("extent_stride", C.c_uint64), ("extent_pages", C.c_uint32), ("page_count", C.c_uint32)]
 
 
+class StepLayout(C.Structure):
+    """rk_step_layout (include/richkv_abi.h)."""
+    _fields_ = [("pool", StepPool), ("lanes", C.c_uint32), ("table_pages", C.c_uint32), ("row_capacity", C.c_uint32),
+                ("split_count", C.c_uint32), ("score_scale", C.c_float), ("reserved", C.c_uint32)]
+
+
+class StepOutputs(C.Structure):
+    """rk_step_outputs (include/richkv_abi.h)."""
+    _fields_ = [("entries", C.c_void_p), ("chunk_params", C.c_void_p), ("verify_params", C.c_void_p), ("row_offsets", C.c_void_p),
+                ("row_slots", C.c_void_p), ("status", C.c_void_p)]
+
+
 class SharedPlan(C.Structure):
     """rk_shared_plan (include/richkv.h)."""
     _fields_ = [("decode", DecodePlan), ("prefix_ctas", C.c_uint32), ("reserved", C.c_uint32),
@@ -115,7 +127,7 @@ SIGNATURES = {
     "rk_attention_decode_shaped": (i32, [vp, C.POINTER(DecodePlan), u32, vp, vp, vp, vp, vp, vp, vp, vp, KvLayer, C.POINTER(ScoreShape), vp]),
     "rk_shared_plan_make": (i32, [u32, u32, u32, u32, u32, u32, C.POINTER(SharedPlan)]),
     "rk_attention_decode_shared": (i32, [vp, C.POINTER(SharedPlan), u32, vp, vp, vp, C.POINTER(SharedBuffers), vp, vp, KvLayer, vp, vp, C.POINTER(ScoreShape), vp]),
-    "rk_step_tables": (i32, [C.POINTER(StepPool), u32, u32, u32, u32, C.c_float, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "rk_step_tables": (i32, [C.POINTER(StepLayout), vp, vp, vp, vp, vp, C.POINTER(StepOutputs), vp]),
     "rk_prefix_groups": (i32, [u32, vp, vp, u32, u32, vp, vp, vp]),
     "rk_attention_decode_shard": (i32, [vp, C.POINTER(DecodePlan), u32, vp, vp, vp, vp, vp, vp, vp, KvLayer, vp]),
     "rk_attention_merge_shards": (i32, [u32, u32, u32, u32, u32, vp, vp, vp, vp]),

@@ -74,10 +74,13 @@ class ScoreShape:
             raise ValueError("ScoreShape: slopes is a contiguous fp32 device vector, one per query head")
         self.softcap, self.window, self.sink_tokens, self.slopes = softcap, window, sink_tokens, slopes
 
+        self._block = lib.ScoreShape(softcap, window, sink_tokens, 0, slopes.data_ptr() if slopes is not None else None)
+
     def block(self, query_heads: int) -> lib.ScoreShape:
+        """The C block; `slopes` stays alive with this object."""
         if self.slopes is not None and self.slopes.numel() != query_heads:
             raise ValueError(f"ScoreShape: {self.slopes.numel()} slopes for {query_heads} query heads")
-        return lib.ScoreShape(self.softcap, self.window, self.sink_tokens, 0, self.slopes.data_ptr() if self.slopes is not None else None)
+        return self._block
 
 
 class VerifyWindowAttention:
@@ -110,7 +113,7 @@ class VerifyWindowAttention:
             status = self._lib.rk_attention_verify_split_shaped(
                 self._window, self.layout.format, self.layout.kv_heads, self.query_heads, self.layout.head_dimension,
                 lanes, row_capacity, grid_splits, queries.data_ptr(), partials.data_ptr(), statistics.data_ptr(),
-                table_pointers.data_ptr(), params.data_ptr(), layer, C.byref(shape.block(self.query_heads)),
+                table_pointers.data_ptr(), params.data_ptr(), layer, shape.block(self.query_heads),
                 self.status_word.data_ptr(), _stream(stream))
             lib.check(status, "rk_attention_verify_split_shaped")
             return
@@ -128,7 +131,7 @@ class VerifyWindowAttention:
             status = self._lib.rk_attention_prefill_split_shaped(
                 self._window, self.layout.format, self.layout.kv_heads, self.query_heads, self.layout.head_dimension,
                 queries.data_ptr(), partials.data_ptr(), statistics.data_ptr(), table.data_ptr(), C.byref(params),
-                C.byref(shape.block(self.query_heads)), self.status_word.data_ptr(), _stream(stream))
+                shape.block(self.query_heads), self.status_word.data_ptr(), _stream(stream))
             lib.check(status, "rk_attention_prefill_split_shaped")
             return
         status = self._lib.rk_attention_prefill_split_tc(
@@ -288,7 +291,7 @@ class DecodeAttention:
                 self._window, C.byref(self.plan), self.layout.format, queries.data_ptr(), output.data_ptr(),
                 output_f32.data_ptr() if output_f32 is not None else None, self.partials.data_ptr(),
                 self.statistics.data_ptr(), self.descriptors.data_ptr(), table_pointers.data_ptr(), params.data_ptr(),
-                layer, C.byref(shape.block(self.query_heads)), _stream(stream))
+                layer, shape.block(self.query_heads), _stream(stream))
             lib.check(status, "rk_attention_decode_shaped")
             return
         status = self._lib.rk_attention_decode(
@@ -302,6 +305,11 @@ class DecodeAttention:
         """Raises if a bounded device wait ran out during the steps launched so far."""
         lib.check(self._lib.rk_attention_decode_status(C.byref(self.plan), self.descriptors.data_ptr(), _stream(stream)),
                   "rk_attention_decode_status")
+
+
+def _int32_vector(name: str, vector, size: int | None, device) -> None:
+    if vector.dtype is not torch.int32 or vector.device != device or not vector.is_contiguous() or (size is not None and vector.numel() != size):
+        raise ValueError(f"{name} is a contiguous int32 vector on {device}" + (f" of {size}" if size is not None else ""))
 
 
 class StepTables:
@@ -318,7 +326,6 @@ class StepTables:
         self._lib = lib.load()
         self.lanes, self.table_pages, self.row_capacity = lanes, table_pages, row_capacity
         self.split_count, self.score_scale = split_count, score_scale
-        self._pool = lib.StepPool(window[0], extent_stride, extent_pages, page_count)
         self.entries = torch.zeros((lanes, table_pages), dtype=torch.int64, device="cuda")
         self.table_pointers = self.entries.data_ptr() + 8 * table_pages * torch.arange(lanes, dtype=torch.int64, device="cuda")
         self.chunk_params = torch.zeros((lanes, CHUNK_PARAMS.itemsize), dtype=torch.uint8, device="cuda")
@@ -326,6 +333,12 @@ class StepTables:
         self.row_offsets = torch.zeros(lanes + 1, dtype=torch.int32, device="cuda")
         self.row_slots = torch.zeros(lanes * row_capacity, dtype=torch.int64, device="cuda")
         self.status_word = torch.zeros(1, dtype=torch.int32, device="cuda")
+        self._device = self.entries.device
+        self._call = self._lib.rk_step_tables
+        self._layout = lib.StepLayout(lib.StepPool(window[0], extent_stride, extent_pages, page_count), lanes, table_pages, row_capacity,
+                                      split_count, score_scale, 0)
+        self._outputs = lib.StepOutputs(*(t.data_ptr() for t in (self.entries, self.chunk_params, self.verify_params, self.row_offsets,
+                                                                 self.row_slots, self.status_word)))
 
     @classmethod
     def for_storage(cls, storage, lanes: int, table_pages: int, row_capacity: int = 1, split_count: int = 1,
@@ -337,20 +350,15 @@ class StepTables:
     def build(self, page_ids, page_offsets, committed, rows, known_pages=None, stream=None) -> None:
         """Per lane l: page ids page_ids[page_offsets[l] : page_offsets[l + 1]], committed tokens, new rows (0: idle);
         entries before known_pages[l] stay as they are. All int32 device vectors."""
-        for name, vector, size in (("page_ids", page_ids, None), ("page_offsets", page_offsets, self.lanes + 1),
-                                   ("committed", committed, self.lanes), ("rows", rows, self.lanes), ("known_pages", known_pages, self.lanes)):
-            if vector is None and name == "known_pages":
-                continue
-            if vector.dtype != torch.int32 or not vector.is_contiguous() or vector.device != self.entries.device or \
-                    (size is not None and vector.numel() != size):
-                raise ValueError(f"StepTables.build: {name} is a contiguous int32 vector on the tables' device" +
-                                 (f" of {size}" if size else ""))
-        status = self._lib.rk_step_tables(
-            C.byref(self._pool), self.lanes, self.table_pages, self.row_capacity, self.split_count, self.score_scale,
-            page_ids.data_ptr(), page_offsets.data_ptr(), committed.data_ptr(), rows.data_ptr(),
-            known_pages.data_ptr() if known_pages is not None else None, self.entries.data_ptr(), self.chunk_params.data_ptr(),
-            self.verify_params.data_ptr(), self.row_offsets.data_ptr(), self.row_slots.data_ptr(), self.status_word.data_ptr(),
-            _stream(stream))
+        lanes, device = self.lanes, self._device
+        _int32_vector("page_ids", page_ids, None, device)
+        _int32_vector("page_offsets", page_offsets, lanes + 1, device)
+        _int32_vector("committed", committed, lanes, device)
+        _int32_vector("rows", rows, lanes, device)
+        if known_pages is not None:
+            _int32_vector("known_pages", known_pages, lanes, device)
+        status = self._call(self._layout, page_ids.data_ptr(), page_offsets.data_ptr(), committed.data_ptr(), rows.data_ptr(),
+                            known_pages.data_ptr() if known_pages is not None else None, self._outputs, _stream(stream))
         lib.check(status, "rk_step_tables")
 
     def check(self) -> None:
@@ -364,9 +372,8 @@ def prefix_groups(lanes: int, table_pointers, params, lane_groups, group_pages, 
                   stream=None) -> None:
     """Which lanes share how long a prefix, from their page tables (rk_prefix_groups): lane_groups[l] = the lowest lane
     of l's group or -1, group_pages[that lane] = the pages they share. Both int32 device vectors of `lanes`."""
-    for name, vector in (("lane_groups", lane_groups), ("group_pages", group_pages)):
-        if vector.dtype != torch.int32 or not vector.is_contiguous() or vector.numel() != lanes:
-            raise ValueError(f"prefix_groups: {name} is a contiguous int32 vector of {lanes}")
+    _int32_vector("lane_groups", lane_groups, lanes, table_pointers.device)
+    _int32_vector("group_pages", group_pages, lanes, table_pointers.device)
     status = lib.load().rk_prefix_groups(lanes, table_pointers.data_ptr(), params.data_ptr(), minimum_lanes, minimum_pages,
                                          lane_groups.data_ptr(), group_pages.data_ptr(), _stream(stream))
     lib.check(status, "rk_prefix_groups")
@@ -394,6 +401,7 @@ class SharedPrefixDecode:
         self.prefix_partials = torch.empty(self.plan.prefix_partials_bytes // 4, dtype=torch.float32, device="cuda")
         self.prefix_statistics = torch.empty(self.plan.prefix_statistics_bytes // 4, dtype=torch.float32, device="cuda")
         self.prefix_descriptors = torch.zeros(self.plan.prefix_descriptor_bytes // 4, dtype=torch.int32, device="cuda")
+        self._device = self.partials.device
         self._buffers = lib.SharedBuffers(*(t.data_ptr() for t in (self.partials, self.statistics, self.descriptors, self.prefix_partials,
                                                                    self.prefix_statistics, self.prefix_descriptors)))
 
@@ -410,13 +418,12 @@ class SharedPrefixDecode:
 
     def run(self, queries, output, table_pointers, params, layer: lib.KvLayer, lane_groups, group_pages, output_f32=None,
             stream=None, shape: ScoreShape | None = None):
-        for name, vector in (("lane_groups", lane_groups), ("group_pages", group_pages)):
-            if vector.dtype != torch.int32 or not vector.is_contiguous() or vector.numel() != self.lanes:
-                raise ValueError(f"SharedPrefixDecode.run: {name} is a contiguous int32 vector of {self.lanes}")
-        block = C.byref(shape.block(self.query_heads)) if shape is not None else None
+        _int32_vector("lane_groups", lane_groups, self.lanes, self._device)
+        _int32_vector("group_pages", group_pages, self.lanes, self._device)
+        block = shape.block(self.query_heads) if shape is not None else None
         status = self._lib.rk_attention_decode_shared(
-            self._window, C.byref(self.plan), self.layout.format, queries.data_ptr(), output.data_ptr(),
-            output_f32.data_ptr() if output_f32 is not None else None, C.byref(self._buffers), table_pointers.data_ptr(),
+            self._window, self.plan, self.layout.format, queries.data_ptr(), output.data_ptr(),
+            output_f32.data_ptr() if output_f32 is not None else None, self._buffers, table_pointers.data_ptr(),
             params.data_ptr(), layer, lane_groups.data_ptr(), group_pages.data_ptr(), block, _stream(stream))
         lib.check(status, "rk_attention_decode_shared")
 

@@ -13,9 +13,8 @@ def step_tables(pool=POOL, lanes=4, table_pages=8, capacity=1, splits=1, missing
     arrays = [16 * (i + 1) for i in range(11)]  # never followed
     if missing is not None:
         arrays[missing] = None
-    ids, offsets, committed, rows, known, entries, chunk, verify, row_offsets, slots, status = arrays
-    return lib.load().rk_step_tables(C.byref(pool) if pool else None, lanes, table_pages, capacity, splits, 0.0, ids, offsets, committed, rows, known,
-                                     entries, chunk, verify, row_offsets, slots, status, None)
+    layout = lib.StepLayout(pool, lanes, table_pages, capacity, splits, 0.0, 0) if pool else None
+    return lib.load().rk_step_tables(layout, *arrays[:5], lib.StepOutputs(*arrays[5:]), None)
 
 
 @pytest.mark.parametrize("change", [dict(lanes=0), dict(lanes=1025), dict(table_pages=0), dict(capacity=0), dict(capacity=17), dict(splits=0),
