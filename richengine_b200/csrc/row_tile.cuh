@@ -225,18 +225,17 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
       // inside every 8 dims, dims 1,5,3,7 divided by 16; int8, fp8: fp16 in order; bf16: the bits. A power of two keeps large
       // queries inside fp16 (exact).
       const uint16_t *query = row.query + part * (kD / kRowThreads);
+      uint4 words[8]; // 64 dims, read once: they become the operands in place
+#pragma unroll
+      for (uint32_t c = 0; c < 8; ++c) words[c] = row.real ? __ldg(reinterpret_cast<const uint4 *>(query + 8 * c)) : make_uint4(0, 0, 0, 0);
       int exponent = 0;
       if (!Kind::kBf16) {
         float amax = 0.0f;
-        if (row.real) {
-#pragma unroll 4
-          for (uint32_t c = 0; c < kD / kRowThreads / 8; ++c) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(query + 8 * c));
-            const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-              amax = fmaxf(amax, fmaxf(fabsf(bf16_bits_to_float(words[i] & 0xffffu)), fabsf(bf16_bits_to_float(words[i] >> 16))));
-          }
+        for (uint32_t c = 0; c < 8; ++c) {
+          const uint32_t w[4] = {words[c].x, words[c].y, words[c].z, words[c].w};
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(bf16_bits_to_float(w[i] & 0xffffu)), fabsf(bf16_bits_to_float(w[i] >> 16))));
         }
         sh.exchange[0][part][my_row] = amax;
         row_barrier();
@@ -244,41 +243,28 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
         for (uint32_t i = 0; i < kRowThreads; ++i) amax = fmaxf(amax, sh.exchange[0][i][my_row]);
         if (amax >= 8192.0f) exponent = ilogbf(amax) - 12;
       }
-      const float down = ldexpf(1.0f, -exponent);
       float q_sum = 0.0f; // over the values the tensor core will see, for the key-offset correction
-      {
-        float columns[32]; // 64 dims
+      if (!Kind::kBf16) {
+        const float down = ldexpf(1.0f, -exponent);
 #pragma unroll
         for (uint32_t c = 0; c < 8; ++c) {
-          uint4 raw = make_uint4(0, 0, 0, 0);
-          if (row.real) raw = __ldg(reinterpret_cast<const uint4 *>(query + 8 * c));
-          const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-          uint32_t chunk[4];
-          if (Kind::kBf16) {
+          const uint32_t w[4] = {words[c].x, words[c].y, words[c].z, words[c].w};
+          float d[8];
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) chunk[i] = words[i];
-          } else {
-            float d[8];
+          for (uint32_t i = 0; i < 4; ++i) { d[2 * i] = bf16_bits_to_float(w[i] & 0xffffu) * down; d[2 * i + 1] = bf16_bits_to_float(w[i] >> 16) * down; }
+          if (Format == RK_FORMAT_INT4)
+            words[c] = make_uint4(pack_half2(d[0], d[4]), pack_half2(d[1] * 0.0625f, d[5] * 0.0625f), pack_half2(d[2], d[6]), pack_half2(d[3] * 0.0625f, d[7] * 0.0625f));
+          else
+            words[c] = make_uint4(pack_half2(d[0], d[1]), pack_half2(d[2], d[3]), pack_half2(d[4], d[5]), pack_half2(d[6], d[7]));
+          const uint32_t h[4] = {words[c].x, words[c].y, words[c].z, words[c].w};
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) { d[2 * i] = bf16_bits_to_float(words[i] & 0xffffu) * down; d[2 * i + 1] = bf16_bits_to_float(words[i] >> 16) * down; }
-            if (Format == RK_FORMAT_INT4) {
-              chunk[0] = pack_half2(d[0], d[4]); chunk[1] = pack_half2(d[1] * 0.0625f, d[5] * 0.0625f);
-              chunk[2] = pack_half2(d[2], d[6]); chunk[3] = pack_half2(d[3] * 0.0625f, d[7] * 0.0625f);
-            } else {
-#pragma unroll
-              for (uint32_t i = 0; i < 4; ++i) chunk[i] = pack_half2(d[2 * i], d[2 * i + 1]);
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-              const __half2 h = *reinterpret_cast<const __half2 *>(&chunk[i]);
-              q_sum += ((Format == RK_FORMAT_INT4 && (i & 1u)) ? 16.0f : 1.0f) * (__low2float(h) + __high2float(h));
-            }
+          for (uint32_t i = 0; i < 4; ++i) {
+            const __half2 pair = *reinterpret_cast<const __half2 *>(&h[i]);
+            q_sum += ((Format == RK_FORMAT_INT4 && (i & 1u)) ? 16.0f : 1.0f) * (__low2float(pair) + __high2float(pair));
           }
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) columns[c * 4 + i] = __uint_as_float(chunk[i]);
         }
-        tmem_store32(tmem_q + lane_address + part * 32, columns);
       }
+      tmem_store32(tmem_q + lane_address + part * 32, reinterpret_cast<const float (&)[32]>(words));
       if (!Kind::kBf16) sh.exchange[1][part][my_row] = q_sum;
       tmem_fence_before();
       warp_arrive(&sh.query_full, lane);
@@ -363,15 +349,29 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
       barrier_wait(&sh.p_free[last & 1u], last >> 1, error);
       tmem_fence_after();
       const bool failed = *error != 0;
+      // Lanes l and l ^ 1 swap halves of 32 bytes, so that each store instruction writes whole sectors: both write the even
+      // lane's row, then both the odd one's.
       float *out = args.partials + row.slot * kD + part * kOutColumns;
+      const bool odd = lane & 1u;
+      float *other_out = reinterpret_cast<float *>(__shfl_xor_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), 1));
+      const bool other_real = __shfl_xor_sync(0xffffffffu, row.real, 1);
+      float *even_out = odd ? other_out + 4 : out, *odd_out = odd ? out + 4 : other_out;
+      const bool even_real = odd ? other_real : row.real, odd_real = odd ? row.real : other_real;
 #pragma unroll 1
       for (uint32_t c = 0; c < kOutColumns; c += 32) {
         float o[32];
         tmem_load32(tmem_o + lane_address + part * kOutColumns + c, o);
-        if (row.real) {
 #pragma unroll
-          for (uint32_t i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4 *>(out + c + i) = make_float4(o[i] * 0.015625f, o[i + 1] * 0.015625f, o[i + 2] * 0.015625f, o[i + 3] * 0.015625f);
+        for (uint32_t i = 0; i < 32; i += 8) {
+          float theirs[4]; // the even lane gives its upper half away, the odd one its lower
+#pragma unroll
+          for (uint32_t e = 0; e < 4; ++e) theirs[e] = __shfl_xor_sync(0xffffffffu, odd ? o[i + e] : o[i + 4 + e], 1);
+          const float4 mine = odd ? make_float4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]) : make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          const float4 given = make_float4(theirs[0], theirs[1], theirs[2], theirs[3]);
+          const float4 even = odd ? given : mine, other = odd ? mine : given;
+          constexpr float kUnscale = 0.015625f; // 2^-6
+          if (even_real) *reinterpret_cast<float4 *>(even_out + c + i) = make_float4(even.x * kUnscale, even.y * kUnscale, even.z * kUnscale, even.w * kUnscale);
+          if (odd_real) *reinterpret_cast<float4 *>(odd_out + c + i) = make_float4(other.x * kUnscale, other.y * kUnscale, other.z * kUnscale, other.w * kUnscale);
         }
       }
       tmem_fence_before();

@@ -71,17 +71,23 @@ __device__ __noinline__ void plan_launch(const PrefixArgs &args, PlanShared &sh)
   for (uint32_t r = 0; r < kRounds; ++r) {
     const uint32_t i = tid + r * kRowTileThreads;
     group[r] = kNone;
-    if (i >= lanes) continue;
-    const uint32_t g = args.lane_groups[i];
-    const rk_verify_params p = args.lane_params[i];
-    const uint32_t shared = g < lanes ? args.group_pages[g] : 0;
-    if (shared && lane_takes_part(p)) {
-      group[r] = g;
-      pages[r] = min(shared, rk_pages_for(p.committed_tokens + 1));
-      atomicAdd(&sh.count[g], 1u);
-      atomicMin(&sh.leader[g], i);
+    if (i / 32 >= words) continue; // the whole warp
+    if (i < lanes) {
+      const uint32_t g = args.lane_groups[i];
+      const rk_verify_params p = args.lane_params[i];
+      const uint32_t shared = g < lanes ? args.group_pages[g] : 0;
+      if (shared && lane_takes_part(p)) {
+        group[r] = g;
+        pages[r] = min(shared, rk_pages_for(p.committed_tokens + 1));
+      }
+      sh.member_of[i] = uint16_t(group[r]);
     }
-    sh.member_of[i] = uint16_t(group[r]);
+    // one pair of atomics per group and warp: every lane on one word would be a queue of 32
+    const uint32_t peers = __match_any_sync(0xffffffffu, group[r]);
+    if (group[r] != kNone && lane == uint32_t(__ffs(peers) - 1)) {
+      atomicAdd(&sh.count[group[r]], uint32_t(__popc(peers)));
+      atomicMin(&sh.leader[group[r]], i);
+    }
   }
   __syncthreads();
   uint32_t members[kRounds];
@@ -227,7 +233,7 @@ shared_merge_kernel(const float *__restrict__ partials, const float *__restrict_
                     const float *__restrict__ prefix_partials, const float *__restrict__ prefix_statistics,
                     const uint4 *__restrict__ prefix_descriptors, uint16_t *__restrict__ output, float *__restrict__ output_f32,
                     const rk_verify_params *__restrict__ lane_params) {
-  constexpr uint32_t kBatch = kGroups == 1 ? 8 : 4;
+  constexpr uint32_t kBatch = kGroups == 4 ? 8 : 4; // slots of a thread in flight: what the registers of its block size allow
   __shared__ float4 sums[kRows][kGroups][kD / 4];
   __shared__ float2 stats[kRows][kGroups];
   const uint32_t head = blockIdx.y, l = blockIdx.z, tid = threadIdx.x, quad = tid & 63u, group = tid / 64 % kGroups, row = tid / (64 * kGroups);
