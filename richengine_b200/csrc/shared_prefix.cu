@@ -239,7 +239,7 @@ shared_merge_kernel(const float *__restrict__ partials, const float *__restrict_
   const uint32_t head = blockIdx.y, l = blockIdx.z, tid = threadIdx.x, quad = tid & 63u, group = tid / 64 % kGroups, row = tid / (64 * kGroups);
   const uint32_t query_head = blockIdx.x * kRows + row;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory"); // the streaming kernel, which itself waited for the prefix kernel
+  asm volatile("griddepcontrol.wait;" ::: "memory"); // the row tiles, whose blocks all waited for the streaming kernel
   const uint2 descriptor = __ldcg(reinterpret_cast<const uint2 *>(descriptors + 2 * l));
   const uint4 prefix = __ldcg(prefix_descriptors + l);
   if (!lane_takes_part(lane_params[l])) return;
@@ -359,11 +359,12 @@ int rk_attention_decode_shared(const void *window, const rk_shared_plan *plan, u
   const PrefixArgs args{{static_cast<const uint16_t *>(queries), buffers->prefix_partials, buffers->prefix_statistics, layer, w->base,
                          buffers->descriptors + 2 * lanes, kSpinLimit, shape_args},
                         buffers->prefix_descriptors, tables, lane_params, lanes, lane_groups, group_pages};
-  int st = launch_row_tile<PrefixPlacement>(format, w, plan->prefix_ctas, args, s);
-  if (st) return st;
-  if ((st = launch_decode_suffix(format, plan->decode, s, w, queries, buffers->partials, buffers->statistics, buffers->descriptors, tables,
-                                 lane_params, layer, shape_args, lane_groups, group_pages)))
+  // The streaming kernel goes first: it leaves its SMs one by one, and the longer prologue of the row tiles (the plan, tensor
+  // memory) runs beside its tail. Neither needs the other; the merge waits for the second, whose blocks all waited for the first.
+  if (int st = launch_decode_suffix(format, plan->decode, s, w, queries, buffers->partials, buffers->statistics, buffers->descriptors, tables,
+                                    lane_params, layer, shape_args, lane_groups, group_pages))
     return st;
+  if (int st = launch_row_tile<PrefixPlacement>(format, w, plan->prefix_ctas, args, s)) return st;
   auto merge = [&](auto kernel, uint32_t rows, uint32_t groups) {
     return launch_dependent(kernel, dim3(kG / rows, kHeads, lanes), 64 * groups * rows, 0, s, "shared merge launch", buffers->partials,
                             buffers->statistics, buffers->descriptors, buffers->prefix_partials, buffers->prefix_statistics,
