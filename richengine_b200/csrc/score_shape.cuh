@@ -34,23 +34,60 @@ inline bool shape_arguments(const rk_score_shape *shape, ShapeArgs &out) {
   return true;
 }
 
+// Two fp32 operations in one instruction, each rounded as on its own.
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
+  float2 r;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+  float2 r;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
 // cap * tanh(s / cap) for N scores, tanh(u) = 1 - 2 / (e^2u + 1). The hardware's own tanh (2^-11) would move a score of 30
-// by 0.015; this form has an absolute error of about cap * 2^-22, two special-function operations per score. Caps up to
-// 256 take it as it is: under 2^-13 on a score, where the weights are rounded to 2^-11. Beyond, scores are small against
-// the cap and the difference from one loses them: below |u| = 1/4 the odd series u (1 - u^2/3 + 2u^4/15 - 17u^6/315 +
-// 62u^8/2835), whose next term is under 10^-8 there, takes over, and the result is good to about 10^-6 of itself.
+// by 0.015; this form has an absolute error of about cap * 2^-22. Four scores share one reciprocal (1/a = b c d / (a b c d)):
+// five special-function operations for four scores instead of eight, which the softmax warps of a 16-row window, short of
+// that unit, pay for. e^2u stops at 2^30, where the quotient is under half a step of one, so that four of them stay finite.
+// Caps up to 256 take this form: its error is under 2^-13 on a score, where the weights are rounded to 2^-11. Beyond, scores
+// are small against the cap and the difference from one loses them: below |u| = 1/4 the odd series u (1 - u^2/3 + 2u^4/15 -
+// 17u^6/315 + 62u^8/2835), whose next term is under 10^-8 there, takes over, and the result is good to about 10^-6 of itself.
 constexpr float kDirectCap = 256.0f * 1.4426950408889634f;
+__device__ __forceinline__ float exp2_special(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_special(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 template <uint32_t N> __device__ __forceinline__ void soft_cap(float (&s)[N], float cap, float cap_inverse) {
+  static_assert(N % 4 == 0, "four scores share a reciprocal");
   const float factor = cap_inverse * 2.8853900817779268f; // e^2u = 2^(2u log2 e)
-  auto far = [&](float x) {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * factor));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
-    return fmaf(-2.0f * cap, r, cap);
-  };
   if (cap <= kDirectCap) { // the same branch for the whole launch
+    const float2 one = make_float2(1.0f, 1.0f), caps = make_float2(cap, cap), down = make_float2(-2.0f * cap, -2.0f * cap);
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) s[i] = far(s[i]);
+    for (uint32_t i = 0; i < N; i += 4) {
+      float e[4];
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) e[k] = exp2_special(fminf(s[i + k] * factor, 30.0f));
+      const float2 a = add_pair(make_float2(e[0], e[1]), one), b = add_pair(make_float2(e[2], e[3]), one), ab = mul_pair(a, b);
+      const float r = reciprocal_special(ab.x * ab.y);
+      const float2 both = make_float2(r * ab.y, r * ab.x); // 1 / ab
+      const float2 low = fma_pair(mul_pair(both, b), down, caps), high = fma_pair(mul_pair(both, a), down, caps);
+      s[i] = low.x; s[i + 1] = low.y; s[i + 2] = high.x; s[i + 3] = high.y;
+    }
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) {
@@ -59,8 +96,8 @@ template <uint32_t N> __device__ __forceinline__ void soft_cap(float (&s)[N], fl
       near = fmaf(u2, near, 0.13333333f);
       near = fmaf(u2, near, -0.33333333f);
       near = fmaf(u2 * s[i], near, s[i]);
-      s[i] = far(s[i]);
-      // a select, not a branch: 64 branches would keep every score's both sides alive (a NaN stays one)
+      s[i] = fmaf(-2.0f * cap, reciprocal_special(exp2_special(s[i] * factor) + 1.0f), cap);
+      // a select, not a branch: branches would keep both sides of every score alive (a NaN stays one)
       asm("{\n.reg .pred p;\nsetp.lt.f32 p, %2, 0f3D800000;\nselp.f32 %0, %1, %0, p;\n}" : "+f"(s[i]) : "f"(near), "f"(u2));
     }
   }

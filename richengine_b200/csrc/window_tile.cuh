@@ -434,25 +434,6 @@ template <> struct Expand<RK_FORMAT_BF16> {
 };
 
 // ---- a softmax thread's N scores of a 64-token group ----------------------------------------------------------------
-// Two fp32 operations in one instruction, each rounded as on its own.
-__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
-  float2 r;
-  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
-  float2 r;
-  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
 // Accumulators to scores + log2(value scale); `position` is the thread's first of the group.
 template <uint32_t N>
 __device__ __forceinline__ void scale_scores(float (&scores)[N], const ScaleStage &stage, uint32_t position, float row_factor, float row_offset) {

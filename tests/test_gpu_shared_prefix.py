@@ -254,3 +254,45 @@ def test_a_whole_step_eager_and_replayed(fmt):
     del graph
     runner.close()
     batch.close()
+
+
+@pytest.mark.parametrize("fmt", [INT4, BF16])
+def test_a_session_that_shares_prefixes(fmt):
+    """DecodeSession: tables from lengths, append and attention of each step through step_device, with the prefix shared and
+    without, with a layer's score shape and without."""
+    from richengine_b200.session import DecodeSession
+    s = Shared(fmt, [(6, 7)], 2, suffix=40)
+    b, shape = s.batch, (9.0, 0, 0, SLOPES)
+    session = DecodeSession(b.storage, 24, s.lanes)
+    tables = session.step_tables(max(map(len, b.pages)))
+    ids, counts = np.concatenate(b.pages).astype(np.int32), [len(p) for p in b.pages]
+    tables.build(dev(ids), dev(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)), dev(np.array(s.committed, np.int32)),
+                 torch.ones(s.lanes, dtype=torch.int32, device="cuda"))
+    rng = np.random.default_rng(3)
+    session.chunk_keys.copy_(dev(make_queries(rng, s.lanes, HEADS, 32, DIM)).view(torch.bfloat16))
+    session.chunk_values.copy_(dev(make_queries(rng, s.lanes, HEADS, DIM, 32)).view(torch.bfloat16))
+    session.queries.copy_(dev(s.queries).view(torch.bfloat16))
+    steps = []
+    for sharing, with_shape in ((False, False), (True, False), (True, True), (False, True)):
+        if sharing:
+            session.share_prefixes(tables.table_pointers, tables.verify_params, minimum_pages=1)
+            assert int(session._group_pages.max()) == 6 and int((session._lane_groups >= 0).sum()) == 7
+        else:
+            session.forget_prefixes()
+        session.output.zero_()
+        session.step_device(0, tables.table_pointers, tables.chunk_params, tables.verify_params, shape=shape_of(shape) if with_shape else None)
+        steps.append((with_shape, host16(session.output)))
+    session.status()
+    tables.check()
+    # by default two lanes over a few pages are not worth a kernel of their own
+    session.share_prefixes(tables.table_pointers, tables.verify_params)
+    assert int(session._group_pages.max()) == 0
+    for extent in range(b.host.extents):
+        b.host.bytes[extent][:] = b.storage.read_extent(extent)
+    for with_shape, got16 in steps:
+        for lane in range(s.lanes):
+            want, bound = b.attend(lane, s.committed[lane], s.queries[lane, :, 0], shape if with_shape else None)
+            got = (got16[lane, :, 0].astype(np.uint32) << 16).view(np.float32)
+            assert (np.abs(got - want) <= bound + 2.0 ** -20 * np.abs(want).max() + np.abs(want) * 2.0 ** -8 + bound * 2.0 ** -8).all()
+    session.close()
+    b.close()
