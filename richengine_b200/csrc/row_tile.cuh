@@ -46,7 +46,7 @@ struct RowPlace {
 
 struct RowTileShared {
   uint64_t raw_full[kMaxRawStages], raw_free[kMaxRawStages];
-  uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], p_free[2], scale_free[kScaleStages];
+  uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], p_free[2];
   uint64_t query_full, output_free, drained[2];
   uint32_t tmem_base;
   uint32_t error;
@@ -93,10 +93,15 @@ __device__ __forceinline__ void shape_scores(float (&scores)[kRowTokens], const 
   if (shape.slopes) {
     const float first = float(int32_t(view.first - position + part_token)), second = float(int32_t(view.second - position + part_token - kPageTokens));
     const float mine = part_token < kPageTokens ? first : second;
+    const float2 slopes = make_float2(slope, slope);
 #pragma unroll
-    for (uint32_t i = 0; i < kRowTokens; ++i) {
-      const float origin = kPermuted ? (local_token<kPermuted>(i) < kPageTokens ? first : second) : mine;
-      scores[i] = fmaf(slope, origin + float(local_token<kPermuted>(i)), scores[i]);
+    for (uint32_t i = 0; i < kRowTokens; i += 2) { // both tokens of a pair lie in one page, unless the order puts them 8 apart at its end
+      const float2 origin = make_float2(kPermuted ? (local_token<kPermuted>(i) < kPageTokens ? first : second) : mine,
+                                        kPermuted ? (local_token<kPermuted>(i + 1) < kPageTokens ? first : second) : mine);
+      const float2 distance = add_pair(origin, make_float2(float(local_token<kPermuted>(i)), float(local_token<kPermuted>(i + 1))));
+      const float2 s = fma_pair(slopes, distance, make_float2(scores[i], scores[i + 1]));
+      scores[i] = s.x;
+      scores[i + 1] = s.y;
     }
   }
 #pragma unroll
@@ -167,7 +172,6 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
       barrier_init(smem_u32(&sh.p_full[b]), kSoftmaxWarps);
       barrier_init(smem_u32(&sh.drained[b]), 1);
     }
-    for (uint32_t b = 0; b < kScaleStages; ++b) barrier_init(smem_u32(&sh.scale_free[b]), kSoftmaxWarps);
     barrier_init(smem_u32(&sh.query_full), kSoftmaxWarps);
     barrier_init(smem_u32(&sh.output_free), kSoftmaxWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -337,7 +341,6 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
         if constexpr (Kind::kBf16) tmem_store_packed(tmem_s + b * 64 + 32 + lane_address + part * (kRowTokens / 2), packed_low);
         tmem_fence_before();
         warp_arrive(&sh.p_full[b], lane);
-        warp_arrive(&sh.scale_free[n % kScaleStages], lane);
       }
 
       // ---- partial output: the row of O, un-normalised, a quarter of its columns by each thread; {reference exponent, sum} ----
@@ -406,7 +409,9 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
         const uint8_t *raw = raw_ptr + r * kRawStageBytes;
         barrier_wait(&sh.raw_full[r], n / kRawStages, error);
         if (e < kGroupTokens) {
-          if (n >= kScaleStages) barrier_wait(&sh.scale_free[n % kScaleStages], n / kScaleStages - 1, error);
+          // The slot's last readers are done: this team wrote the values of group n - kTileStages once the contraction of the
+          // group kTileStages before that had landed, which is n - kScaleStages or later, and its weights came from those scales.
+          static_assert(2 * kTileStages <= kScaleStages, "a scale slot outlives its readers");
           const uint32_t token = Expand<Format>::token_of(e);
           float key_scale = 0.0f, value_log = 0.0f, factor = 0.0f;
           if (valid.holds(token)) {

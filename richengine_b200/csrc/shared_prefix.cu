@@ -20,7 +20,6 @@ constexpr uint32_t kMaxLanes = 1024;
 constexpr uint32_t kNone = 0xffffu;
 constexpr uint32_t kTileLanes = 24;   // lanes with a row in a 128-row tile: at most 23
 static_assert(kTileLanes == sizeof(RowItem::lanes) / sizeof(uint16_t), "an item names its tile's lanes");
-constexpr uint32_t kLeastUnits = 4;   // 64-token groups of a split: shorter ones cost more in partials than they spread
 
 struct PrefixArgs : RowTileArgs { // partials [row][256], statistics [row]{max, sum}, rows as the lanes' descriptors say
   uint32_t *descriptors; // [lane]{row of head 0 and split 0, splits, rows of the group, -}
@@ -59,7 +58,8 @@ __device__ __forceinline__ uint32_t bits_before(const uint32_t *words, uint32_t 
 }
 
 // How the launch is cut, the same in every CTA: members per group, the groups with work, and the shortest split length for
-// which (KV heads x tiles x splits) of all groups still fit the grid. With more tiles than CTAs every tile is one item and
+// which (KV heads x tiles x splits) of all groups still fit the grid (down to one 64-token group: a longer chain of groups
+// costs more than the partials that the merge reads; four lanes over 2K tokens: 25.8 us, and 29.1 with four groups at least). With more tiles than CTAs every tile is one item and
 // the CTAs take them in turn.
 __device__ __noinline__ void plan_launch(const PrefixArgs &args, PlanShared &sh) {
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32, lanes = args.lanes, words = (lanes + 31) / 32;
@@ -128,8 +128,8 @@ __device__ __noinline__ void plan_launch(const PrefixArgs &args, PlanShared &sh)
     // items(chunk) <= units / chunk + tiles, and >= units / chunk: the shortest chunk that fits lies between these two
     uint32_t high = units_of(rk_pages_for(RK_MAX_PHYSICAL_TOKENS));
     if (tiles < gridDim.x) {
-      high = max(kLeastUnits, units / (gridDim.x - tiles) + 1);
-      uint32_t low = max(kLeastUnits, (units + gridDim.x - 1) / gridDim.x);
+      high = units / (gridDim.x - tiles) + 1;
+      uint32_t low = max(1u, (units + gridDim.x - 1) / gridDim.x);
       while (low < high) {
         const uint32_t middle = (low + high) / 2;
         if (items_for(middle) <= gridDim.x) high = middle; else low = middle + 1;

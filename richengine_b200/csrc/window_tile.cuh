@@ -117,7 +117,9 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
 // or at once when another wait of this CTA already gave up; either way `error` ends non-zero.
 // `error` points at Control::error; the word after it holds the poll limit of this launch.
 __device__ __forceinline__ void barrier_wait(uint64_t *barrier, uint32_t count, volatile uint32_t *error) {
-  const uint32_t bar = smem_u32(barrier), parity = count & 1u, limit = error[1];
+  const uint32_t bar = smem_u32(barrier), parity = count & 1u;
+  if (barrier_try(bar, parity)) return;
+  const uint32_t limit = error[1];
   for (uint32_t i = 0; i < limit; ++i) {
     if (barrier_try(bar, parity)) return; // try_wait itself suspends the thread for a while
     if ((i & 63u) == 63u) {
