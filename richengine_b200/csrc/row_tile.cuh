@@ -12,13 +12,20 @@
 //   warp 27           the plan: descriptions of the CTA's items, up to eight at a time
 // Tensor memory (512 columns): O 256, two score buffers of 64 (a group's weights overwrite the first half of its scores; of
 // bf16, a low part of each weight the second), the query tile 128.
+//
+// What bounds it: a 64-token group of int4 takes about 2 480 cycles, of which the matrix unit is busy 1 024 (the two
+// contractions at M128), the four schedulers 1 490 (61 % of all issue slots: softmax of 128 x 64 scores, expansion of 32 K
+// codes) and shared memory about 1 450 (operand tiles written and read back, raw codes, scales). Without the softmax the
+// 256-lane prefix takes 188 us instead of 222, without the expansion 205, without either 157: no single part hides the rest,
+// the handoffs between them do. Sixteen softmax warps because eight were latency bound (a group's chain of load, maximum,
+// weights and store is shorter with 16 scores a thread than with 32); two teams of eight that alternate between groups, and a
+// single score buffer beside two of weights, were 4-6 % slower. Rates: 770 TFLOP/s for 256 lanes of int4, 460 for a 16-row
+// window with a soft cap (96 of 128 rows), 545 for a prefill chunk of int8 with a window of 4 096.
 #pragma once
 
 #include "common.cuh"
 #include "score_shape.cuh"
 #include "window_tile.cuh"
-
-#include <string>
 
 namespace rk::tile {
 
@@ -409,8 +416,8 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
         const uint8_t *raw = raw_ptr + r * kRawStageBytes;
         barrier_wait(&sh.raw_full[r], n / kRawStages, error);
         if (e < kGroupTokens) {
-          // The slot's last readers are done: this team wrote the values of group n - kTileStages once the contraction of the
-          // group kTileStages before that had landed, which is n - kScaleStages or later, and its weights came from those scales.
+          // The slot's last readers, the softmax of group n - kScaleStages, are done: before this team expanded the values of
+          // its last group it waited for the contraction two of its groups ago, which is that group's or a later one.
           static_assert(2 * kTileStages <= kScaleStages, "a scale slot outlives its readers");
           const uint32_t token = Expand<Format>::token_of(e);
           float key_scale = 0.0f, value_log = 0.0f, factor = 0.0f;

@@ -6,7 +6,10 @@
 // and KV head, stand side by side as the M side of a tensor-core tile: pages are read once per tile, not once per lane,
 // and a group of n lanes turns 6 multiply-adds per key element into 6 n.
 //
-// The kernel is the row-tile kernel (row_tile.cuh) with rows gathered from many lanes.
+// The kernel is the row-tile kernel (row_tile.cuh) with rows gathered from many lanes. Measured, streaming kernel and merge
+// included: int4, 256 lanes over one 32K prefix 272 us (770 TFLOP/s; 1 364 us lane by lane), 32 over 8K 52 us (61), four over
+// 2K tokens of int8 25 us (20): three launches cost more than four short lanes' pages do. The crossover is near 200 MB of
+// pages saved.
 #include "common.cuh"
 #include "decode_partials.cuh"
 #include "row_tile.cuh"
@@ -58,9 +61,9 @@ __device__ __forceinline__ uint32_t bits_before(const uint32_t *words, uint32_t 
 }
 
 // How the launch is cut, the same in every CTA: members per group, the groups with work, and the shortest split length for
-// which (KV heads x tiles x splits) of all groups still fit the grid (down to one 64-token group: a longer chain of groups
-// costs more than the partials that the merge reads; four lanes over 2K tokens: 25.8 us, and 29.1 with four groups at least). With more tiles than CTAs every tile is one item and
-// the CTAs take them in turn.
+// which (KV heads x tiles x splits) of all groups still fit the grid. It goes down to one 64-token group: a longer chain of
+// groups costs more than the partials that the merge reads (four lanes over 2K tokens: 25 us, and 29 with four groups at
+// least). With more tiles than CTAs every tile is one item and the CTAs take them in turn.
 __device__ __noinline__ void plan_launch(const PrefixArgs &args, PlanShared &sh) {
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32, lanes = args.lanes, words = (lanes + 31) / 32;
   constexpr uint32_t kRounds = (kMaxLanes + kRowTileThreads - 1) / kRowTileThreads; // warps take whole words: lane i of round r is tid + r * kRowTileThreads

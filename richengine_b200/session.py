@@ -69,8 +69,8 @@ class DecodeSession:
     def share_prefixes(self, table_pointers, verify_params, minimum_pages: int | None = None, stream=None) -> None:
         """Finds which lanes share how long a prefix; until the next call (or forget_prefixes) the device steps read every
         shared prefix once. To be called when the batch changes: a group's pages must stay full and shared. By default a
-        group has to be able to save kWorthBytes of pages a layer, about what the extra kernel and merge cost (a B200: 28
-        against 16 us for 4 lanes over 2K int8 tokens, 53 against 60 for 32 over 8K int4, 280 against 1 390 for 256 over 32K)."""
+        group has to be able to save kWorthBytes of pages a layer, about what the extra kernel and merge cost (a B200: 25
+        against 20 us for 4 lanes over 2K int8 tokens, 52 against 61 for 32 over 8K int4, 272 against 1 364 for 256 over 32K)."""
         if minimum_pages is None:
             saved = max(1, self.lanes - 1) * self.layout.bytes_per_layer_page()
             minimum_pages = max(1, -(-self.kWorthBytes // saved))

@@ -177,6 +177,26 @@ def test_verify(fmt, name, rows, capacity, splits):
     batch.close()
 
 
+@pytest.mark.parametrize("fmt", [INT4, BF16])
+def test_verify_of_many_lanes(fmt):
+    """1 920 tiles, heads and splits: more per SM than it plans at a time, lanes without rows and splits without pages
+    among them."""
+    rng = np.random.default_rng(12)
+    contexts = [int(c) for c in rng.integers(0, 150, 160)]
+    rows = [int(r) for r in rng.integers(0, 9, 160)]
+    batch, q = prepared(fmt, contexts, 8, seed=12)
+    shape = (9.0, 60, 3, SLOPES)
+    got16, got32 = verify(batch, contexts, rows, 8, q, shape_of(shape), 3)
+    for lane in range(0, 160, 9):
+        for r in sorted({0, rows[lane] - 1} & set(range(8))):
+            if r < rows[lane]:
+                want, bound = batch.attend(lane, contexts[lane] + r, q[lane, :, r], shape)
+                check_rows(got32[lane, :, r], got16[lane, :, r], want, bound, f"lane {lane}, row {r}")
+    for lane in range(160):
+        assert not got16[lane, :, rows[lane]:].any()
+    batch.close()
+
+
 # ---- prefill tiles --------------------------------------------------------------------------------------------------
 
 def prefill(batch, committed, rows, queries, shape, splits):
@@ -208,6 +228,41 @@ def test_prefill(fmt, name, committed, rows, splits):
     for r in sorted({0, 7, 8, rows // 2, rows - 1} & set(range(rows))):
         want, bound = batch.attend(0, committed + r, q[:, r], shape)
         check_rows(got32[:, r], got16[:, r], want, bound, f"{name}, row {r}")
+    batch.close()
+
+
+@pytest.mark.parametrize("fmt", [INT8, FP8E4M3])
+def test_prefill_of_many_tiles(fmt):
+    """1 280 tiles, heads and splits: more per SM than it plans at a time."""
+    committed, rows, shape = 90, 320, (0.0, 70, 2, SLOPES)
+    batch, _ = prepared(fmt, [committed], rows)
+    q = make_queries(np.random.default_rng(3), HEADS, rows, GROUP, DIM)
+    got16, got32 = prefill(batch, committed, rows, q, shape_of(shape), splits=8)
+    for r in range(0, rows, 29):
+        want, bound = batch.attend(0, committed + r, q[:, r], shape)
+        check_rows(got32[:, r], got16[:, r], want, bound, f"row {r}")
+    batch.close()
+
+
+@pytest.mark.parametrize("shift16,shift32", [(1, 0), (0, 1), (3, 2)])
+def test_merges_into_rows_at_any_address(shift16, shift32):
+    """Outputs that start between the words the merge would like to write: the same bits."""
+    contexts, rows, splits = [0, 100, 333], 5, 4
+    batch, _ = prepared(INT4, contexts, rows)
+    params = batch.params(contexts, rows, 8, splits)
+    prefill_params = lib.PrefillParams(100, 21, 32, 8, batch.layer, splits, 0.0)
+    generator = torch.Generator("cuda").manual_seed(1)
+    partials = torch.randn(3 * HEADS * splits * 8 * GROUP * DIM, device="cuda", generator=generator)
+    statistics = torch.rand(3 * HEADS * splits * 8 * GROUP * 2, device="cuda", generator=generator)
+    for shape, merge in (((3, HEADS, 32, GROUP, DIM), lambda o, f: ops.attention_verify_reduce(batch.layout, 24, 3, 8, partials, statistics, o, params, output_f32=f)),
+                         ((HEADS, 32, GROUP, DIM), lambda o, f: ops.attention_prefill_reduce(batch.layout, 24, partials, statistics, o, prefill_params, output_f32=f))):
+        size, results = int(np.prod(shape)), []
+        for a, b in ((0, 0), (shift16, shift32)):
+            out, out32 = torch.zeros(size + 8, dtype=torch.bfloat16, device="cuda"), torch.zeros(size + 8, device="cuda")
+            merge(out[a:a + size].view(shape), out32[b:b + size].view(shape))
+            assert not out[:a].any() and not out[a + size:].any() and not out32[:b].any() and not out32[b + size:].any()
+            results.append((out[a:a + size].clone(), out32[b:b + size].clone()))
+        assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1]) and results[0][1].any()
     batch.close()
 
 

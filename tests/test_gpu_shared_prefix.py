@@ -86,6 +86,16 @@ def test_against_64_bits(fmt, name):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("ctas", [1, 2])
+def test_many_items_per_block(fmt, ctas):
+    """24 tiles and heads on one or two CTAs: each takes more of them than it plans at a time."""
+    groups, loose = GROUPS["a tile and its neighbours"]
+    s = Shared(fmt, groups, loose, suffix=40)
+    s.check(*s.run(ctas=ctas), lanes=range(0, s.lanes, 9))
+    s.batch.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("shape", [(4.0, 0, 0, None), (0.0, 0, 0, SLOPES), (0.0, 60, 3, None), (6.0, 150, 40, SLOPES), (0.0, 1, 0, None)])
 def test_with_a_score_shape(fmt, shape):
     s = Shared(fmt, [(5, 6), (3, 2)], 2)
