@@ -167,7 +167,9 @@ int rk_attention_decode(const void *window, const rk_decode_plan *plan, uint32_t
                         uint32_t *descriptors, const rk_page_entry *const *tables,
                         const rk_verify_params *lane_params, rk_kv_layer layer, void *stream);
 /* No counterpart in the reference. rk_attention_decode with a score shape (rk_score_shape): only the pages with a token
- * that the row sees are read. Plan, scratch and status word as for rk_attention_decode. */
+ * that the row sees are read. Plan, scratch and status word as for rk_attention_decode. Here and below, the key and value
+ * rows of tokens that a row sees have to be finite (a soft cap turns a score that is no number into the cap); what the
+ * others hold does not matter. */
 int rk_attention_decode_shaped(const void *window, const rk_decode_plan *plan, uint32_t format, const void *queries,
                                void *output, float *output_f32, float *partials, float *statistics,
                                uint32_t *descriptors, const rk_page_entry *const *tables,
@@ -180,7 +182,9 @@ int rk_attention_decode_shaped(const void *window, const rk_decode_plan *plan, u
  * lane_groups[l] (a number below `lanes`; anything else: no group) and group g shares its first group_pages[g] pages, which
  * are the same in every member's table and full of tokens that every member has committed. `shape` may be null. Scratch
  * is sized by the plan; the caller zeroes buffers->descriptors once, and its status word (rk_attention_decode_status
- * with &plan->decode) covers both kernels. At most 1 024 lanes. */
+ * with &plan->decode) covers both kernels. lane_params, lane_groups and group_pages are read as soon as the launch before
+ * lets its dependents start: they must not come from a kernel that does so before it has written them (rk_step_tables and
+ * rk_prefix_groups do not). At most 1 024 lanes. */
 typedef struct rk_shared_plan {
   rk_decode_plan decode;
   uint32_t prefix_ctas, reserved;
@@ -305,7 +309,8 @@ int rk_step_tables(const rk_step_layout *layout, const uint32_t *page_ids, const
  * count). Lanes are gathered under the lowest lane that has their first page; of those, the ones that share the p pages
  * for which (lanes - 1) * p is largest (ties: the larger p) become a group, if there are at least minimum_lanes (>= 2) of
  * them and p >= minimum_pages. lane_groups[l] = the group's lowest lane, or RK_NO_GROUP; group_pages[l] = p at a group's
- * lowest lane, 0 elsewhere. Both [lanes], device memory. At most 1 024 lanes. */
+ * lowest lane, 0 elsewhere. Both [lanes], device memory. Lanes that every kernel skips (no live rows) belong to no group.
+ * At most 1 024 lanes. */
 int rk_prefix_groups(uint32_t lanes, const rk_page_entry *const *tables, const rk_verify_params *lane_params,
                      uint32_t minimum_lanes, uint32_t minimum_pages, uint32_t *lane_groups, uint32_t *group_pages,
                      void *stream);

@@ -339,6 +339,7 @@ class StepTables:
                                       split_count, score_scale, 0)
         self._outputs = lib.StepOutputs(*(t.data_ptr() for t in (self.entries, self.chunk_params, self.verify_params, self.row_offsets,
                                                                  self.row_slots, self.status_word)))
+        torch.cuda.current_stream().synchronize()  # the fills above are done, whichever stream the first call takes
 
     @classmethod
     def for_storage(cls, storage, lanes: int, table_pages: int, row_capacity: int = 1, split_count: int = 1,
@@ -404,6 +405,7 @@ class SharedPrefixDecode:
         self._device = self.partials.device
         self._buffers = lib.SharedBuffers(*(t.data_ptr() for t in (self.partials, self.statistics, self.descriptors, self.prefix_partials,
                                                                    self.prefix_statistics, self.prefix_descriptors)))
+        torch.cuda.current_stream().synchronize()  # the fills above are done, whichever stream the first call takes
 
     def close(self):
         if self._window:

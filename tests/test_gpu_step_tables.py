@@ -227,3 +227,20 @@ def test_group_refusals():
             ops.prefix_groups(*arguments)
     with pytest.raises(ValueError, match="lane_groups"):
         ops.prefix_groups(3, lanes, lanes, lanes, lanes)
+
+
+def test_the_first_call_may_take_another_stream():
+    """Made under a busy stream and built on an idle one at once: the object's own fills are over."""
+    busy, idle = torch.cuda.Stream(), torch.cuda.Stream()
+    inputs = [i32(v) for v in ([3, 1], [0, 1, 2], [5, 9], [1, 1])]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(50_000_000)
+        tables = ops.StepTables(2, 4, (1 << 40, 1 << 20), 1 << 16, 2, 8)
+    tables.build(*inputs, stream=idle)
+    with torch.cuda.stream(idle):
+        pointers, slots = tables.table_pointers.clone(), tables.row_slots.clone()
+    idle.synchronize()
+    assert pointers.tolist() == [tables.entries.data_ptr(), tables.entries.data_ptr() + 32] and slots.tolist() == [101, 41]
+    torch.cuda.synchronize()
+    assert tables.row_slots.tolist() == [101, 41]
