@@ -76,15 +76,36 @@ struct RowTileArgs {
 };
 
 // ---- a softmax thread's scores --------------------------------------------------------------------------------------------
-// Accumulators of contraction positions first_position .. + 15 to scores + log2(value scale), the unseen ones -infinity.
-// part_token: what those positions add to local_token<...>(i) of the first sixteen.
+// Adds slope * (token - the group's first token) to the scores and returns slope * (the group's first token - position).
 template <bool kPermuted>
-__device__ __forceinline__ void shape_scores(float (&scores)[kRowTokens], const ScaleStage &stage, uint32_t first_position, uint32_t part_token,
+__device__ __forceinline__ float bias_scores(float (&scores)[kRowTokens], uint32_t part_token, float slope, const GroupView &view, uint32_t position) {
+  const float gap = slope * float(int32_t(view.second - view.first - kPageTokens)); // zero unless the list skips pages between the two
+#pragma unroll
+  for (uint32_t i = 0; i < kRowTokens; ++i) scores[i] = fmaf(slope, float(local_token<kPermuted>(i)), scores[i]);
+  float origin = slope * float(int32_t(view.first + part_token - position));
+  if (!kPermuted && part_token >= kPageTokens) origin += gap;
+  if (kPermuted && gap != 0.0f) {
+#pragma unroll
+    for (uint32_t i = 0; i < kRowTokens; ++i)
+      if (local_token<kPermuted>(i) >= kPageTokens) scores[i] += gap;
+  }
+  return origin;
+}
+// Accumulators of contraction positions first_position .. + 15 to scores + log2(value scale), the unseen ones -infinity.
+// part_token: what those positions add to local_token<...>(i) of the first sixteen. Of a bias -slope * (position - token), the
+// part that these tokens have in common (by their page, which is one page or two neighbours) is returned, to be added by the
+// caller once instead of sixteen times; the rest is one multiply-add by a constant per score.
+template <bool kPermuted>
+__device__ __forceinline__ float shape_scores(float (&scores)[kRowTokens], const ScaleStage &stage, uint32_t first_position, uint32_t part_token,
                                              float row_factor, float row_offset, const ShapeArgs &shape, float slope, const GroupView &view,
                                              uint32_t position) {
   if (shape.cap == 0.0f && !shape.slopes) { // one branch for the launch
     scale_scores(scores, stage, first_position, row_factor, row_offset);
-    return;
+    return 0.0f;
+  }
+  if (shape.cap == 0.0f) {
+    scale_scores(scores, stage, first_position, row_factor, row_offset);
+    return bias_scores<kPermuted>(scores, part_token, slope, view, position);
   }
   const float2 factor = make_float2(row_factor, row_factor), offset = make_float2(row_offset, row_offset);
   float2 logs[kRowTokens / 2];
@@ -96,27 +117,14 @@ __device__ __forceinline__ void shape_scores(float (&scores)[kRowTokens], const 
     scores[i + 1] = s.y;
     logs[i / 2] = make_float2(pair.z, pair.w);
   }
-  if (shape.cap > 0.0f) soft_cap(scores, shape.cap, shape.cap_inverse);
-  if (shape.slopes) {
-    const float first = float(int32_t(view.first - position + part_token)), second = float(int32_t(view.second - position + part_token - kPageTokens));
-    const float mine = part_token < kPageTokens ? first : second;
-    const float2 slopes = make_float2(slope, slope);
-#pragma unroll
-    for (uint32_t i = 0; i < kRowTokens; i += 2) { // both tokens of a pair lie in one page, unless the order puts them 8 apart at its end
-      const float2 origin = make_float2(kPermuted ? (local_token<kPermuted>(i) < kPageTokens ? first : second) : mine,
-                                        kPermuted ? (local_token<kPermuted>(i + 1) < kPageTokens ? first : second) : mine);
-      const float2 distance = add_pair(origin, make_float2(float(local_token<kPermuted>(i)), float(local_token<kPermuted>(i + 1))));
-      const float2 s = fma_pair(slopes, distance, make_float2(scores[i], scores[i + 1]));
-      scores[i] = s.x;
-      scores[i + 1] = s.y;
-    }
-  }
+  soft_cap(scores, shape.cap, shape.cap_inverse);
 #pragma unroll
   for (uint32_t i = 0; i < kRowTokens; i += 2) {
     const float2 s = add_pair(make_float2(scores[i], scores[i + 1]), logs[i / 2]);
     scores[i] = s.x;
     scores[i + 1] = s.y;
   }
+  return shape.slopes ? bias_scores<kPermuted>(scores, part_token, slope, view, position) : 0.0f;
 }
 template <bool kPermuted>
 __device__ __forceinline__ void mask_scores(float (&scores)[kRowTokens], uint32_t part_token, uint32_t seen_first, uint32_t seen_second) {
@@ -301,13 +309,14 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
         tmem_fence_after();
         float scores[kRowTokens];
         tmem_load_scores(tmem_s + b * 64 + lane_address + first_position, scores);
-        shape_scores<kPermuted>(scores, stage, first_position, part_token, row_factor, row_offset, args.shape, slope, view, position);
+        const float common = shape_scores<kPermuted>(scores, stage, first_position, part_token, row_factor, row_offset, args.shape, slope, view, position);
         // Most groups are seen whole by every row of a warp: nothing is tested then.
         if (!__all_sync(0xffffffffu, view.whole(position, row_window)))
           mask_scores<kPermuted>(scores, part_token, view.seen_first(position, row_window, sinks), view.seen_second(position, row_window, sinks));
         float maximum = scores[0];
 #pragma unroll
         for (uint32_t i = 1; i < kRowTokens; ++i) maximum = fmaxf(maximum, scores[i]);
+        maximum += common;
         // the row's other parts; past this barrier every part holds its scores in registers, so the weights may overwrite the
         // first 32 columns of the buffer
         sh.exchange[b][part][my_row] = maximum;
@@ -324,7 +333,7 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
           row_max = maximum;
           row_sum *= scale;
         }
-        weigh_scores(scores, stage, first_position, row_max - 6.0f, row_sum);
+        weigh_scores(scores, stage, first_position, row_max - 6.0f - common, row_sum);
         uint32_t packed[kRowTokens / 2], packed_low[Kind::kBf16 ? kRowTokens / 2 : 1];
 #pragma unroll
         for (uint32_t c = 0; c < kRowTokens / 2; ++c) {
