@@ -13,14 +13,16 @@
 // Tensor memory (512 columns): O 256, two score buffers of 64 (a group's weights overwrite the first half of its scores; of
 // bf16, a low part of each weight the second), the query tile 128.
 //
-// What bounds it: a 64-token group of int4 takes about 2 480 cycles, of which the matrix unit is busy 1 024 (the two
-// contractions at M128), the four schedulers 1 490 (61 % of all issue slots: softmax of 128 x 64 scores, expansion of 32 K
-// codes) and shared memory about 1 450 (operand tiles written and read back, raw codes, scales). Without the softmax the
-// 256-lane prefix takes 188 us instead of 222, without the expansion 205, without either 157: no single part hides the rest,
-// the handoffs between them do. Sixteen softmax warps because eight were latency bound (a group's chain of load, maximum,
+// What bounds it: a 64-token group of int4 takes about 2 400 cycles, of which the matrix unit is busy 1 024 (the two
+// contractions at M128), the schedulers 1 450 (61 % of all issue slots: softmax of 128 x 64 scores, expansion of 32 K codes)
+// and shared memory about 2 100 (1 450 wavefronts of loads and stores, half of them scales that every row's thread reads, 128
+// of the copies in, 512 of the matrix unit's operand reads). Work left out in a copy: without the softmax the 256-lane prefix
+// takes 188 us instead of 222, without the expansion 205, without either 157, without the scales' reads 205: several limits
+// lie close together. What a shape adds to the softmax shows in full (a cap 26 us of 85, slopes 20 % of a prefill chunk).
+// Sixteen softmax warps because eight were latency bound (a group's chain of load, maximum,
 // weights and store is shorter with 16 scores a thread than with 32); two teams of eight that alternate between groups, and a
 // single score buffer beside two of weights, were 4-6 % slower. Rates: 770 TFLOP/s for 256 lanes of int4, 460 for a 16-row
-// window with a soft cap (96 of 128 rows), 545 for a prefill chunk of int8 with a window of 4 096.
+// window with a soft cap (96 of 128 rows), 570 for a prefill chunk of int8 with slopes and a window of 4 096.
 #pragma once
 
 #include "common.cuh"

@@ -57,7 +57,7 @@ __device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
 // cap * tanh(s / cap) for N scores, tanh(u) = 1 - 2 / (e^2u + 1). The hardware's own tanh (2^-11) would move a score of 30
 // by 0.015; this form has an absolute error of about cap * 2^-22. Four scores share one reciprocal (1/a = b c d / (a b c d)):
 // five special-function operations for four scores instead of eight, in the softmax warps of a 16-row window, which are
-// short of that unit (four lanes over 32K int4 tokens: 115 us, and 121 with a reciprocal each; 90 without a cap). e^2u stops at 2^30, where the quotient is under half a step of one, so that four of them stay finite.
+// short of that unit (four lanes over 32K int4 tokens: 115 us, and 121 with a reciprocal each; 86 without a cap). e^2u stops at 2^30, where the quotient is under half a step of one, so that four of them stay finite.
 // Caps up to 256 take this form: its error is under 2^-13 on a score, where the weights are rounded to 2^-11. Beyond, scores
 // are small against the cap and the difference from one loses them: below |u| = 1/4 the odd series u (1 - u^2/3 + 2u^4/15 -
 // 17u^6/315 + 62u^8/2835), whose next term is under 10^-8 there, takes over, and the result is good to about 10^-6 of itself.

@@ -5,9 +5,9 @@
 // merges count the splits that exist from the whole context, so the listed pages are dealt to that many, in whole 64-token
 // groups, and a split that gets none leaves an empty partial.
 //
-// Measured: four lanes of 16 rows over 32K int4 tokens with a soft cap 112 us with the merge (90 without a shape's work, 86
-// on the plain window kernel, which needs no plan); 2 048 int8 rows behind 6K with a window of 4 096 380 us, of which the
-// merge is 24 (without a shape 511 us; the plain prefill kernel takes 584 for the same rows).
+// Measured: four lanes of 16 rows over 32K int4 tokens with a soft cap 112 us with the merge (86 with an empty shape, 83 on
+// the plain window kernel, which needs no plan); 2 048 int8 rows behind 6K with a window of 4 096 and slopes 362 us, of
+// which the merge is 24 (with an empty shape 484 us; the plain prefill kernel takes 564 for the same rows).
 #include "row_tile.cuh"
 
 #include <atomic>
