@@ -22,8 +22,8 @@ from .abi import CHUNK_PARAMS, TREE_NODES, VERIFY_PARAMS, Layout
 
 
 def _stream(stream) -> int:
-    if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+    if stream is None:  # the current stream's handle without a Stream object around it: 0.3 us of a call instead of 3.2
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 

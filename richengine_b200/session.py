@@ -26,9 +26,7 @@ from .storage import PageStorage
 
 
 def _stream_handle(stream) -> int:
-    if stream is None:
-        return torch.cuda.current_stream().cuda_stream
-    return stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
+    return ops._stream(stream)
 
 
 class DecodeSession:
