@@ -180,7 +180,8 @@ int rk_attention_decode_shaped(const void *window, const rk_decode_plan *plan, u
  * contraction; what a lane has behind them streams as in rk_attention_decode; one merge joins both. lane_groups and
  * group_pages are device arrays of one word per lane, as rk_prefix_groups leaves them: lane l belongs to group
  * lane_groups[l] (a number below `lanes`; anything else: no group) and group g shares its first group_pages[g] pages, which
- * are the same in every member's table and full of tokens that every member has committed. `shape` may be null. Scratch
+ * are the same in every member's table and full of tokens that every member has committed. `shape` may be null; with a
+ * window, only the shared pages with a token that some member sees are read. Scratch
  * is sized by the plan; the caller zeroes buffers->descriptors once, and its status word (rk_attention_decode_status
  * with &plan->decode) covers both kernels. lane_params, lane_groups and group_pages are read as soon as the launch before
  * lets its dependents start: they must not come from a kernel that does so before it has written them (rk_step_tables and

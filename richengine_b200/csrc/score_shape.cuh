@@ -103,7 +103,7 @@ template <uint32_t N> __device__ __forceinline__ void soft_cap(float (&s)[N], fl
   }
 }
 
-// The pages that rows at positions first_position..last_position read, as a list: page(o) for o < count. Pages before
+// The pages of tokens 0..last_position that rows at first_position and later read, as a list: page(o) for o < count. Pages before
 // `skip` belong to someone else (a shared prefix); of the rest, those with a sink token and those from the first row's
 // window on.
 struct PageList {
@@ -115,7 +115,8 @@ struct PageList {
     list.window_first = shape.window && first_position + 1 > shape.window ? first_position + 1 - shape.window : 0;
     list.begin = min(skip, pages);
     const uint32_t sinks_end = max(list.begin, rk_pages_for(min(shape.sinks, last_position + 1)));
-    const uint32_t window_begin = max(list.begin, list.window_first / kPageTokens);
+    // (The first row may lie behind the last position and its window with it: then the list keeps the last page, seen by none.)
+    const uint32_t window_begin = max(list.begin, min(list.window_first / kPageTokens, pages - 1));
     if (window_begin <= sinks_end) {
       list.head = list.count = pages - list.begin;
       list.gap = 0;

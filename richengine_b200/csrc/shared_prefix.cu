@@ -32,8 +32,15 @@ struct PrefixArgs : RowTileArgs { // partials [row][256], statistics [row]{max, 
   const uint32_t *lane_groups, *group_pages;
 };
 
-// A group with work: its number, members and pages, and the lowest member's lane (whose table the tiles read).
-struct GroupWork { uint16_t group, members, pages, leader; };
+// A group with work: its number, members and pages, the lowest member's lane (whose table the tiles read), and the smallest
+// position of its rows, whose window begins first.
+struct GroupWork {
+  uint16_t group, members, pages, leader;
+  uint32_t nearest;
+  __device__ __forceinline__ uint32_t last_position() const { return pages * kPageTokens - 1; }
+  // the pages of the prefix that some row sees
+  __device__ __forceinline__ PageList list(const ShapeArgs &shape) const { return PageList::make(nearest, last_position(), 0, shape); }
+};
 
 struct PlanShared {
   uint16_t member_of[kMaxLanes];  // a lane's group, kNone: none
@@ -41,6 +48,7 @@ struct PlanShared {
     struct {
       uint32_t count[kMaxLanes];  // members of a group
       uint32_t leader[kMaxLanes]; // its lowest member
+      uint32_t nearest[kMaxLanes]; // its smallest position
     };
     GroupWork list[kMaxLanes];    // then: the groups with work, by leader
   };
@@ -67,7 +75,7 @@ __device__ __forceinline__ uint32_t bits_before(const uint32_t *words, uint32_t 
 __device__ __noinline__ void plan_launch(const PrefixArgs &args, PlanShared &sh) {
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32, lanes = args.lanes, words = (lanes + 31) / 32;
   constexpr uint32_t kRounds = (kMaxLanes + kRowTileThreads - 1) / kRowTileThreads; // warps take whole words: lane i of round r is tid + r * kRowTileThreads
-  for (uint32_t i = tid; i < lanes; i += kRowTileThreads) { sh.count[i] = 0; sh.leader[i] = kMaxLanes; }
+  for (uint32_t i = tid; i < lanes; i += kRowTileThreads) { sh.count[i] = 0; sh.leader[i] = kMaxLanes; sh.nearest[i] = ~0u; }
   __syncthreads();
   uint32_t group[kRounds], pages[kRounds]; // of this thread's lanes
 #pragma unroll
@@ -82,6 +90,7 @@ __device__ __noinline__ void plan_launch(const PrefixArgs &args, PlanShared &sh)
       if (shared && lane_takes_part(p)) {
         group[r] = g;
         pages[r] = min(shared, rk_pages_for(p.committed_tokens + 1));
+        if (args.shape.window) atomicMin(&sh.nearest[g], p.committed_tokens);
       }
       sh.member_of[i] = uint16_t(group[r]);
     }
@@ -93,12 +102,13 @@ __device__ __noinline__ void plan_launch(const PrefixArgs &args, PlanShared &sh)
     }
   }
   __syncthreads();
-  uint32_t members[kRounds];
+  uint32_t members[kRounds], nearest[kRounds];
 #pragma unroll
   for (uint32_t r = 0; r < kRounds; ++r) {
     const uint32_t i = tid + r * kRowTileThreads;
     if (i / 32 >= words) continue; // the whole warp
     members[r] = group[r] != kNone ? sh.count[group[r]] : 0;
+    nearest[r] = group[r] != kNone ? sh.nearest[group[r]] : 0;
     const uint32_t mask = __ballot_sync(0xffffffffu, group[r] != kNone && sh.leader[group[r]] == i);
     if (lane == 0) sh.words[i / 32] = mask;
   }
@@ -108,7 +118,7 @@ __device__ __noinline__ void plan_launch(const PrefixArgs &args, PlanShared &sh)
     const uint32_t i = tid + r * kRowTileThreads;
     if (i / 32 >= words) continue;
     const uint32_t mask = sh.words[i / 32], at = bits_before(sh.words, i / 32) + __popc(mask & ((1u << lane) - 1u));
-    if (mask >> lane & 1u) sh.list[at] = GroupWork{uint16_t(group[r]), uint16_t(members[r]), uint16_t(pages[r]), uint16_t(i)};
+    if (mask >> lane & 1u) sh.list[at] = GroupWork{uint16_t(group[r]), uint16_t(members[r]), uint16_t(pages[r]), uint16_t(i), nearest[r]};
     if (i / 32 + 1 == words && lane == 31) sh.groups = at + (mask >> 31);
   }
   __syncthreads();
@@ -118,14 +128,14 @@ __device__ __noinline__ void plan_launch(const PrefixArgs &args, PlanShared &sh)
     for (uint32_t i = lane; i < groups; i += 32) {
       const uint32_t t = kHeads * tiles_of(sh.list[i].members);
       tiles += t;
-      units += t * units_of(sh.list[i].pages);
+      units += t * units_of(sh.list[i].list(args.shape).count);
     }
     units = __reduce_add_sync(0xffffffffu, units);
     tiles = __reduce_add_sync(0xffffffffu, tiles);
     auto items_for = [&](uint32_t chunk) {
       uint32_t sum = 0;
       for (uint32_t i = lane; i < groups; i += 32)
-        sum += kHeads * tiles_of(sh.list[i].members) * ((units_of(sh.list[i].pages) + chunk - 1) / chunk);
+        sum += kHeads * tiles_of(sh.list[i].members) * ((units_of(sh.list[i].list(args.shape).count) + chunk - 1) / chunk);
       return __reduce_add_sync(0xffffffffu, sum);
     };
     // items(chunk) <= units / chunk + tiles, and >= units / chunk: the shortest chunk that fits lies between these two
@@ -162,8 +172,9 @@ struct PrefixPlacement : PlanShared {
     uint32_t before = 0, rows = 0;
     for (uint32_t base = 0; base < groups; base += 32) {
       const bool live = base + lane < groups;
-      const GroupWork work = live ? list[base + lane] : GroupWork{0, 0, 0, 0};
-      const uint32_t units = units_of(work.pages), splits = (units + chunk - 1) / chunk, tiles = tiles_of(work.members);
+      const GroupWork work = live ? list[base + lane] : GroupWork{0, 0, 1, 0, 0};
+      const PageList pages = work.list(args.shape);
+      const uint32_t units = units_of(pages.count), splits = (units + chunk - 1) / chunk, tiles = tiles_of(work.members);
       const uint32_t items = kHeads * tiles * splits, group_rows = work.members * kG;
       uint32_t items_up = items, rows_up = kHeads * splits * group_rows;
 #pragma unroll
@@ -177,9 +188,9 @@ struct PrefixPlacement : PlanShared {
           const uint32_t within = index - (before + items_up - items), split = within / kHeads / tiles, tile = within / kHeads % tiles;
           item.head = within % kHeads;
           item.ordinal_begin = 2 * (units * split / splits);
-          item.ordinal_end = min(uint32_t(work.pages), 2 * (units * (split + 1) / splits));
-          item.list = PageList{0, work.pages, 0, work.pages, 0};
-          item.last_position = work.pages * kPageTokens - 1;
+          item.ordinal_end = min(pages.count, 2 * (units * (split + 1) / splits));
+          item.list = pages;
+          item.last_position = work.last_position();
           item.table = args.tables[work.leader];
           item.place[0] = tile;
           item.place[1] = split;

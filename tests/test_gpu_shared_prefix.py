@@ -103,6 +103,27 @@ def test_with_a_score_shape(fmt, shape):
     s.batch.close()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("shape", [(0.0, 200, 40, None), (0.0, 90, 0, SLOPES), (0.0, 10, 33, None), (7.0, 1000, 1, None)])
+@pytest.mark.parametrize("ctas", [0, 3])
+def test_prefix_pages_outside_every_window_are_not_read(fmt, shape, ctas):
+    """Prefixes longer than the window: pages that no member sees are 0xFF throughout, NaN where the format or its scales
+    have one. Some members see the prefix's end, some only its sinks, some nothing of it."""
+    _, window, sinks, _ = shape
+    s = Shared(fmt, [(40, 6), (9, 30), (3, 2)], 2, suffix=150)
+    seen = {page for lane, pages in enumerate(s.batch.pages) for j, page in enumerate(pages)
+            if j * PAGE < sinks or (j + 1) * PAGE + window > s.committed[lane] + 1}
+    poisoned = {page for pages in s.batch.pages for page in pages} - seen
+    assert window == 1000 or poisoned
+    for page in poisoned:
+        for tensor in range(4):
+            view = s.batch.host.tensor_view(page, 0, tensor)
+            view.view(np.uint8)[:] = 0xff
+    s.batch.upload()
+    s.check(*s.run(shape, ctas=ctas), shape, lanes=range(0, s.lanes, 5))
+    s.batch.close()
+
+
 @pytest.mark.parametrize("fmt", [INT4, BF16])
 def test_equals_the_plain_decode(fmt):
     """The same batch without its groups is rk_attention_decode's business: same rows up to the bound, and bit for bit
