@@ -168,8 +168,8 @@ int rk_attention_decode(const void *window, const rk_decode_plan *plan, uint32_t
                         const rk_verify_params *lane_params, rk_kv_layer layer, void *stream);
 /* No counterpart in the reference. rk_attention_decode with a score shape (rk_score_shape): only the pages with a token
  * that the row sees are read. Plan, scratch and status word as for rk_attention_decode. Here and below, the key and value
- * rows of tokens that a row sees have to be finite (a soft cap turns a score that is no number into the cap); what the
- * others hold does not matter. */
+ * rows of tokens that a row sees have to be finite; what the others hold does not matter. A query row with an element that
+ * is no number comes out as zeros, with a shape and without, as from the other entries. */
 int rk_attention_decode_shaped(const void *window, const rk_decode_plan *plan, uint32_t format, const void *queries,
                                void *output, float *output_f32, float *partials, float *statistics,
                                uint32_t *descriptors, const rk_page_entry *const *tables,

@@ -314,19 +314,19 @@ __device__ __forceinline__ void page_softmax(const float (&sacc)[2][2][4], const
                                              const ShapedPage *shaped = nullptr) {
   float s2[2][2][2], lv[2][2];
   float local_max[2] = {-INFINITY, -INFINITY};
-  float shaped_scores[8];
+  float shaped_scores[8]; // [query head of the pair][token]: the four that share a reciprocal in the cap are of one row
   if (Shaped) {
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
-      const uint32_t mt = i >> 2, half = (i >> 1) & 1u, j = i & 1u;
-      shaped_scores[i] = fmaf(sacc[mt][0][half * 2 + j] + sacc[mt][1][half * 2 + j], hfac[j], negoff[j]) *
-                         load_shared_f32(scales + (16 * mt + 8 * half + r3g) * 4);
+      const uint32_t j = i >> 2, mt = (i >> 1) & 1u, half = i & 1u, token = 16 * mt + 8 * half + r3g;
+      const float score = fmaf(sacc[mt][0][half * 2 + j] + sacc[mt][1][half * 2 + j], hfac[j], negoff[j]) * load_shared_f32(scales + token * 4);
+      shaped_scores[i] = !Masked || ((shaped->seen >> token) & 1u) ? score : 0.0f;
     }
     if (shaped->cap > 0.0f) soft_cap(shaped_scores, shaped->cap, shaped->cap_inverse);
     if (shaped->sloped) {
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i)
-        shaped_scores[i] = fmaf(shaped->slope[i & 1u], float(16 * (i >> 2) + 8 * ((i >> 1) & 1u)) + shaped->distance, shaped_scores[i]);
+        shaped_scores[i] = fmaf(shaped->slope[i >> 2], float(16 * ((i >> 1) & 1u) + 8 * (i & 1u)) + shaped->distance, shaped_scores[i]);
     }
   }
 #pragma unroll
@@ -342,7 +342,7 @@ __device__ __forceinline__ void page_softmax(const float (&sacc)[2][2][4], const
 #pragma unroll
       for (uint32_t j = 0; j < 2; ++j) {
         const float acc = sacc[mt][0][half * 2 + j] + sacc[mt][1][half * 2 + j];
-        const float score = live ? (Shaped ? shaped_scores[4 * mt + 2 * half + j] : fmaf(acc, hfac[j], negoff[j]) * ks) : -INFINITY;
+        const float score = live ? (Shaped ? shaped_scores[4 * j + 2 * mt + half] : fmaf(acc, hfac[j], negoff[j]) * ks) : -INFINITY;
         s2[mt][half][j] = score;
         local_max[j] = fmaxf(local_max[j], score + floor_lv);
       }

@@ -129,12 +129,12 @@ __device__ __forceinline__ float shape_scores(float (&scores)[kRowTokens], const
   return shape.slopes ? bias_scores<kPermuted>(scores, part_token, slope, view, position) : 0.0f;
 }
 template <bool kPermuted>
-__device__ __forceinline__ void mask_scores(float (&scores)[kRowTokens], uint32_t part_token, uint32_t seen_first, uint32_t seen_second) {
+__device__ __forceinline__ void mask_scores(float (&scores)[kRowTokens], uint32_t part_token, uint32_t seen_first, uint32_t seen_second, float unseen) {
   const uint32_t mine = part_token < kPageTokens ? seen_first : seen_second;
 #pragma unroll
   for (uint32_t i = 0; i < kRowTokens; ++i) {
     const uint32_t bits = kPermuted ? (local_token<kPermuted>(i) < kPageTokens ? seen_first : seen_second) : mine;
-    if (!((bits >> ((local_token<kPermuted>(i) + part_token) & 31u)) & 1u)) scores[i] = -INFINITY;
+    if (!((bits >> ((local_token<kPermuted>(i) + part_token) & 31u)) & 1u)) scores[i] = unseen;
   }
 }
 
@@ -311,10 +311,13 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
         tmem_fence_after();
         float scores[kRowTokens];
         tmem_load_scores(tmem_s + b * 64 + lane_address + first_position, scores);
-        const float common = shape_scores<kPermuted>(scores, stage, first_position, part_token, row_factor, row_offset, args.shape, slope, view, position);
         // Most groups are seen whole by every row of a warp: nothing is tested then.
-        if (!__all_sync(0xffffffffu, view.whole(position, row_window)))
-          mask_scores<kPermuted>(scores, part_token, view.seen_first(position, row_window, sinks), view.seen_second(position, row_window, sinks));
+        const bool whole = __all_sync(0xffffffffu, view.whole(position, row_window));
+        if (!whole && args.shape.cap != 0.0f) // the cap wants numbers, also where a row does not look
+          mask_scores<kPermuted>(scores, part_token, view.seen_first(position, row_window, sinks), view.seen_second(position, row_window, sinks), 0.0f);
+        const float common = shape_scores<kPermuted>(scores, stage, first_position, part_token, row_factor, row_offset, args.shape, slope, view, position);
+        if (!whole)
+          mask_scores<kPermuted>(scores, part_token, view.seen_first(position, row_window, sinks), view.seen_second(position, row_window, sinks), -INFINITY);
         float maximum = scores[0];
 #pragma unroll
         for (uint32_t i = 1; i < kRowTokens; ++i) maximum = fmaxf(maximum, scores[i]);

@@ -61,10 +61,18 @@ __device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
 // Caps up to 256 take this form: its error is under 2^-13 on a score, where the weights are rounded to 2^-11. Beyond, scores
 // are small against the cap and the difference from one loses them: below |u| = 1/4 the odd series u (1 - u^2/3 + 2u^4/15 -
 // 17u^6/315 + 62u^8/2835), whose next term is under 10^-8 there, takes over, and the result is good to about 10^-6 of itself.
+// A score that is no number stays one, and takes the three that share its reciprocal with it: callers pass scores of one query
+// row, s[4i] .. s[4i + 3], and give tokens that the row does not see (their keys may hold anything) a finite score beforehand.
 constexpr float kDirectCap = 256.0f * 1.4426950408889634f;
 __device__ __forceinline__ float exp2_special(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// The smaller of two, a NaN when either is one (fminf would return the other).
+__device__ __forceinline__ float minimum_or_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 __device__ __forceinline__ float reciprocal_special(float x) {
@@ -81,7 +89,7 @@ template <uint32_t N> __device__ __forceinline__ void soft_cap(float (&s)[N], fl
     for (uint32_t i = 0; i < N; i += 4) {
       float e[4];
 #pragma unroll
-      for (uint32_t k = 0; k < 4; ++k) e[k] = exp2_special(fminf(s[i + k] * factor, 30.0f));
+      for (uint32_t k = 0; k < 4; ++k) e[k] = exp2_special(minimum_or_nan(s[i + k] * factor, 30.0f));
       const float2 a = add_pair(make_float2(e[0], e[1]), one), b = add_pair(make_float2(e[2], e[3]), one), ab = mul_pair(a, b);
       const float r = reciprocal_special(ab.x * ab.y);
       const float2 both = make_float2(r * ab.y, r * ab.x); // 1 / ab

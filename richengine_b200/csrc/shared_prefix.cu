@@ -311,8 +311,9 @@ shared_merge_kernel(const float *__restrict__ partials, const float *__restrict_
       denominator += weight * own.y;
     }
   }
-  const float inverse = denominator > 0.0f ? 1.0f / denominator : 0.0f;
-  const float4 value = make_float4(numerator.x * inverse, numerator.y * inverse, numerator.z * inverse, numerator.w * inverse);
+  // as the other merges: a row without a positive sum (nothing seen, or no number) is zeros
+  const float4 value = denominator > 0.0f ? make_float4(numerator.x / denominator, numerator.y / denominator, numerator.z / denominator, numerator.w / denominator)
+                                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   const uint64_t at = (uint64_t(l) * kHeads + head) * (RK_VERIFY_CHUNK_STRIDE * kG * kD) + query_head * kD + 4 * quad;
   *reinterpret_cast<uint2 *>(output + at) = make_uint2(uint32_t(float_to_bf16_bits(value.x)) | uint32_t(float_to_bf16_bits(value.y)) << 16,
                                                        uint32_t(float_to_bf16_bits(value.z)) | uint32_t(float_to_bf16_bits(value.w)) << 16);

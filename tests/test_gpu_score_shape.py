@@ -282,3 +282,51 @@ def test_refusals():
             ops.ScoreShape(slopes=slopes)
     runner.close()
     batch.close()
+
+
+# ---- queries that are no numbers ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("shape", [None, (0.0, 0, 0, None), (20.0, 0, 0, None), (256.0, 50, 3, SLOPES), (1.0e4, 0, 0, None)])
+def test_a_query_row_that_is_no_number_comes_out_as_zeros(fmt, shape):
+    """One element of one query head is NaN: that row is zeros, with a shape and without, and its neighbours (the other head of its
+    pair, the other rows of its tile) are what they are without it."""
+    contexts, head, sibling = [40, 700, 333], 2, 5
+    batch, q = prepared(fmt, contexts, 8)
+    block = None if shape is None else shape_of(shape)
+    clean = q.copy()
+    q[1, head, 0, sibling, 7] = 0x7fc0
+    got16, got32 = decode(batch, contexts, q, block)
+    for lane, context in enumerate(contexts):
+        want, bound = batch.attend(lane, context, clean[lane, :, 0], shape)
+        if lane == 1:
+            assert not got16[lane, head, 0, sibling].any() and not got32[lane, head, 0, sibling].any()
+            got16[lane, head, 0, sibling], got32[lane, head, 0, sibling] = 0, want[head, sibling]
+            assert np.isfinite(got32).all()
+            check_rows(got32[lane, :, 0], None, want, bound, f"lane {lane}")
+        else:
+            check_rows(got32[lane, :, 0], got16[lane, :, 0], want, bound, f"lane {lane}")
+    if shape is None:
+        batch.close()
+        return
+    # row 3 of an eight-row window, and of a prefill chunk
+    q = clean.copy()
+    q[1, head, 3, sibling, 200] = 0xffc0
+    got16, got32 = verify(batch, contexts, 8, 8, q, block, splits=3)
+    chunk16, chunk32 = prefill(Lane(batch, 1), contexts[1], 8, q[1], block, splits=1)
+    for r in range(8):
+        want, bound = batch.attend(1, contexts[1] + r, clean[1, :, r], shape)
+        for row32, row16, what in ((got32[1, :, r], got16[1, :, r], "verify"), (chunk32[:, r], chunk16[:, r], "prefill")):
+            if r == 3:
+                assert not row16[head, sibling].any() and not row32[head, sibling].any(), what
+                row32[head, sibling] = want[head, sibling]
+            check_rows(row32, None, want, bound, f"{what}, row {r}")
+    batch.close()
+
+
+class Lane:
+    """One lane of a batch as a batch of its own, for `prefill`."""
+
+    def __init__(self, batch, lane):
+        self.layout, self.layer, self.storage = batch.layout, batch.layer, batch.storage
+        self.pages, self.tables = [batch.pages[lane]], [batch.tables[lane]]

@@ -327,3 +327,22 @@ def test_a_session_that_shares_prefixes(fmt):
             assert (np.abs(got - want) <= bound + 2.0 ** -20 * np.abs(want).max() + np.abs(want) * 2.0 ** -8 + bound * 2.0 ** -8).all()
     session.close()
     b.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("shape", [None, (20.0, 0, 0, None), (300.0, 0, 0, SLOPES)])
+def test_a_query_row_that_is_no_number_comes_out_as_zeros(fmt, shape):
+    s = Shared(fmt, [(5, 6)], 2)
+    clean = s.queries.copy()
+    grouped, loose = s.member.index(0), s.member.index(-1)
+    for lane in (grouped, loose):
+        s.queries[lane, 1, 0, 3, 100] = 0x7fc0
+    got16, got32 = s.run(shape)
+    s.queries = clean
+    for lane in (grouped, loose):
+        assert not got16[lane, 1, 0, 3].any() and not got32[lane, 1, 0, 3].any()
+        want, bound = s.batch.attend(lane, s.committed[lane], clean[lane, :, 0], shape)
+        got32[lane, 1, 0, 3] = want[1, 3]
+        check_rows(got32[lane, :, 0], None, want, bound + 2.0 ** -20 * np.abs(want).max(), f"lane {lane}")
+    s.check(got16, got32, shape, lanes=[l for l in range(s.lanes) if l not in (grouped, loose)])
+    s.batch.close()
