@@ -296,12 +296,13 @@ int rk_session_status(void *session, void *stream);
  * parameter blocks the host would upload. Inputs in device memory, per lane: its pages page_ids[page_offsets[l] ..
  * page_offsets[l + 1]), its committed tokens and the `rows` this step appends (0: idle). Written: entries [lane][table_pages]
  * for the pages that committed + rows tokens need, from known_pages[l] on (null: from 0; entries before it and behind the
- * last needed page stay as they are); the parameter blocks of rk_store_verify and of the decode / verify kernels (their kv
+ * last needed page stay as they are, and all of an idle lane's); the parameter blocks of rk_store_verify and of the decode / verify kernels (their kv
  * fields are zero: the layer is a launch argument there); row_offsets [lanes + 1], the running sum of the rows; and
  * row_slots [row_offsets[lanes]], each new row's place page id * 32 + token in page. `tables` stays the caller's: the
  * address of each lane's row of `entries`. A lane that asks for more rows than row_capacity, more tokens than a sequence
- * may have, more pages than it names or the table holds, or names a page past page_count is made idle (no live rows: every
- * kernel skips it; its slots are all ones) and raises the sticky `status` word. Every page named has to lie in an extent
+ * may have, more pages than it names or the table holds, names a page past page_count, or whose offsets fall or reach past
+ * the id_count ids is made idle (no live rows: every kernel skips it; its slots are all ones) and raises the sticky `status`
+ * word; of such a lane's entries some may have been written. Every page named has to lie in an extent
  * that the pool holds. At most 1 024 lanes; row_slots takes lanes * row_capacity words. */
 int rk_step_tables(const rk_step_layout *layout, const uint32_t *page_ids, const uint32_t *page_offsets,
                    const uint32_t *committed, const uint32_t *rows, const uint32_t *known_pages,

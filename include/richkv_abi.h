@@ -114,12 +114,13 @@ typedef struct rk_step_pool {
   uint32_t extent_pages, page_count;
 } rk_step_pool;
 
-/* What a batch's step tables look like (rk_step_tables): the same from step to step. */
+/* What a batch's step tables look like (rk_step_tables): the same from step to step. id_count: how many page ids there
+ * are, against which page_offsets are checked (0: not known, the offsets are trusted). */
 typedef struct rk_step_layout {
   rk_step_pool pool;
   uint32_t lanes, table_pages, row_capacity, split_count;
   float score_scale;
-  uint32_t reserved; /* 0 */
+  uint32_t id_count;
 } rk_step_layout;
 
 /* Where they go (device memory): entries [lane][table_pages], one parameter block of each kind per lane, row_offsets

@@ -44,9 +44,10 @@ step_tables_kernel(const __grid_constant__ StepArgs a) {
   const uint32_t known = a.known_pages ? a.known_pages[l] : 0;
   uint32_t before = 0; // rows of the lanes before this one
   for (uint32_t i = tid; i < l; i += kTableThreads) before += min(a.rows[i], capacity);
-  const uint32_t count = end >= begin ? end - begin : 0;
+  const bool named = end >= begin && (!a.layout.id_count || end <= a.layout.id_count); // its ids lie in the array
+  const uint32_t count = named ? end - begin : 0;
   const uint64_t tokens = uint64_t(committed) + rows;
-  bool good = rows > 0 && rows <= capacity && end >= begin && tokens <= RK_MAX_PHYSICAL_TOKENS &&
+  bool good = rows > 0 && rows <= capacity && named && tokens <= RK_MAX_PHYSICAL_TOKENS &&
               rk_pages_for(uint32_t(tokens)) <= min(count, a.layout.table_pages);
   const uint32_t pages = good ? rk_pages_for(uint32_t(tokens)) : 0;
   const uint32_t *ids = a.page_ids + begin;

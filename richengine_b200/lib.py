@@ -60,7 +60,7 @@ class StepPool(C.Structure):
 class StepLayout(C.Structure):
     """rk_step_layout (include/richkv_abi.h)."""
     _fields_ = [("pool", StepPool), ("lanes", C.c_uint32), ("table_pages", C.c_uint32), ("row_capacity", C.c_uint32),
-                ("split_count", C.c_uint32), ("score_scale", C.c_float), ("reserved", C.c_uint32)]
+                ("split_count", C.c_uint32), ("score_scale", C.c_float), ("id_count", C.c_uint32)]
 
 
 class StepOutputs(C.Structure):

@@ -350,7 +350,8 @@ class StepTables:
 
     def build(self, page_ids, page_offsets, committed, rows, known_pages=None, stream=None) -> None:
         """Per lane l: page ids page_ids[page_offsets[l] : page_offsets[l + 1]], committed tokens, new rows (0: idle);
-        entries before known_pages[l] stay as they are. All int32 device vectors."""
+        entries before known_pages[l] stay as they are, and all of an idle lane's. All int32 device vectors. A lane whose offsets
+        reach past page_ids is refused like one that asks for too much."""
         lanes, device = self.lanes, self._device
         _int32_vector("page_ids", page_ids, None, device)
         _int32_vector("page_offsets", page_offsets, lanes + 1, device)
@@ -358,6 +359,7 @@ class StepTables:
         _int32_vector("rows", rows, lanes, device)
         if known_pages is not None:
             _int32_vector("known_pages", known_pages, lanes, device)
+        self._layout.id_count = page_ids.numel()
         status = self._call(self._layout, page_ids.data_ptr(), page_offsets.data_ptr(), committed.data_ptr(), rows.data_ptr(),
                             known_pages.data_ptr() if known_pages is not None else None, self._outputs, _stream(stream))
         lib.check(status, "rk_step_tables")

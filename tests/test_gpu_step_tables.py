@@ -111,6 +111,27 @@ def test_the_page_of_a_new_row_is_looked_at_among_the_known_ones_too():
     assert tables.row_slots.cpu().tolist() == [-1]
 
 
+def test_offsets_past_the_page_ids_are_refused():
+    """page_ids is the middle of a longer vector of good ids: a lane whose offsets leave it, on either side, is idle and writes no
+    entry; its neighbours are what they are alone."""
+    around = i32([7] * 40)
+    page_ids = around[16:22]
+    page_ids.copy_(i32([3, 4, 5, 6, 8, 9]))
+    offsets = [(0, 2), (2, 7), (7, 8), (-4, 2), (2 ** 32 - 2, 2 ** 32 - 1), (5, 4), (4, 6)]
+    for begin, end in offsets:
+        tables = ops.StepTables(2, 4, (BASE, 1 << 30), EXTENT_STRIDE, EXTENT_PAGES, 100)
+        # lane 1 has what the pair says; lane 0 whatever ends where that begins
+        tables.build(page_ids, i32([min(begin % 2 ** 32, 1), begin % 2 ** 32, end % 2 ** 32]), i32([0, 0]), i32([0, 1]))
+        live = np.frombuffer(tables.verify_params.cpu().numpy().tobytes(), VERIFY_PARAMS)
+        good = 0 <= begin <= end <= 6
+        assert live["active_rows"].tolist() == [0, int(good)] and live["page_table_entries"][1] == (end - begin if good else 0)
+        assert tables.entries[1].tolist() == ([entry(int(page_ids[begin])), 0, 0, 0] if good else [0] * 4)
+        if not good:
+            with pytest.raises(lib.RichKvError, match="rk_step_tables"):
+                tables.check()
+        tables.check()
+
+
 @pytest.mark.parametrize("fmt", [1, 2, 3, 4])
 def test_entries_equal_the_storage_s_own(fmt):
     """Against rk_storage_entry for pages of every extent (an extent's address range is rounded up to the mapping's grain)."""
