@@ -365,9 +365,12 @@ class StepTables:
         lib.check(status, "rk_step_tables")
 
     def check(self) -> None:
-        """Synchronises, raises if a lane was refused since the last check, and clears the word."""
+        """Waits for the device (whichever streams the builds took, eagerly or in a replayed graph), raises if a lane was refused
+        since the last check, and clears the word."""
+        torch.cuda.synchronize(self._device)
         if int(self.status_word.item()):
             self.status_word.zero_()
+            torch.cuda.current_stream(self._device).synchronize()  # a build on another stream may follow at once
             raise lib.RichKvError(lib.INVALID, "rk_step_tables: a lane asks for rows, tokens or pages it cannot have")
 
 

@@ -265,3 +265,21 @@ def test_the_first_call_may_take_another_stream():
     assert pointers.tolist() == [tables.entries.data_ptr(), tables.entries.data_ptr() + 32] and slots.tolist() == [101, 41]
     torch.cuda.synchronize()
     assert tables.row_slots.tolist() == [101, 41]
+
+
+def test_check_waits_for_the_stream_of_the_build():
+    """A refusal still on its way on another stream is not missed, and the word is clear before a build anywhere follows."""
+    tables = ops.StepTables(1, 4, (BASE, 1 << 30), EXTENT_STRIDE, EXTENT_PAGES, 100)
+    bad, good = ([i32(v) for v in ([3, 4], [0, 2], [c], [1])] for c in (70, 5))
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(200_000_000)
+    tables.build(*bad, stream=other)
+    with pytest.raises(lib.RichKvError, match="rk_step_tables"):
+        tables.check()
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(50_000_000)
+    tables.build(*good, stream=other)
+    tables.check()
+    assert tables.row_slots.tolist() == [3 * 32 + 5]
