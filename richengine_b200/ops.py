@@ -333,6 +333,7 @@ class StepTables:
         self.row_offsets = torch.zeros(lanes + 1, dtype=torch.int32, device="cuda")
         self.row_slots = torch.zeros(lanes * row_capacity, dtype=torch.int64, device="cuda")
         self.status_word = torch.zeros(1, dtype=torch.int32, device="cuda")
+        self._no_ids = torch.full((1,), -1, dtype=torch.int32, device="cuda")  # what an empty page_ids stands for: past every pool
         self._device = self.entries.device
         self._call = self._lib.rk_step_tables
         self._layout = lib.StepLayout(lib.StepPool(window[0], extent_stride, extent_pages, page_count), lanes, table_pages, row_capacity,
@@ -359,6 +360,8 @@ class StepTables:
         _int32_vector("rows", rows, lanes, device)
         if known_pages is not None:
             _int32_vector("known_pages", known_pages, lanes, device)
+        if not page_ids.numel():
+            page_ids = self._no_ids
         self._layout.id_count = page_ids.numel()
         status = self._call(self._layout, page_ids.data_ptr(), page_offsets.data_ptr(), committed.data_ptr(), rows.data_ptr(),
                             known_pages.data_ptr() if known_pages is not None else None, self._outputs, _stream(stream))

@@ -283,3 +283,17 @@ def test_check_waits_for_the_stream_of_the_build():
     tables.build(*good, stream=other)
     tables.check()
     assert tables.row_slots.tolist() == [3 * 32 + 5]
+
+
+def test_a_batch_without_pages():
+    """Every lane idle and no page named: an empty vector of ids will do; a lane that asks for a row all the same is refused."""
+    for rows in ([0, 0], [0, 1]):
+        tables = ops.StepTables(2, 4, (BASE, 1 << 30), EXTENT_STRIDE, EXTENT_PAGES, 100)
+        for offsets in ([0, 0, 0], [0, 0, 1]):
+            tables.build(i32([]), i32(offsets), i32([0, 0]), i32(rows))
+            live = np.frombuffer(tables.verify_params.cpu().numpy().tobytes(), VERIFY_PARAMS)
+            assert live["active_rows"].tolist() == [0, 0] and tables.row_offsets.tolist() == [0, 0, rows[1]] and not tables.entries.any()
+            if rows[1]:
+                with pytest.raises(lib.RichKvError, match="rk_step_tables"):
+                    tables.check()
+            tables.check()
