@@ -141,7 +141,8 @@ int rk_attention_prefill_split_tc(const void *window, uint32_t format, uint32_t 
                                   const rk_page_entry *table, const rk_prefill_params *params, uint32_t *status,
                                   void *stream);
 /* No counterparts in the reference. The two calls above with a score shape (rk_score_shape): chain windows of 8 or 16
- * rows and prefill tiles, every format; scratch, split counts and merges are theirs. A window's CTA reads only the pages
+ * rows and prefill tiles, every format; scratch, split counts and merges are theirs. Queries and partials start on 16-byte
+ * boundaries, statistics and tables on 8-byte ones; others are refused. A window's CTA reads only the pages
  * with a token that one of its rows sees; the key and value rows of those tokens have to be finite. */
 int rk_attention_verify_split_shaped(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,
                                      uint32_t head_dim, uint32_t lanes, uint32_t row_capacity, uint32_t grid_splits,
@@ -167,7 +168,9 @@ int rk_attention_decode(const void *window, const rk_decode_plan *plan, uint32_t
                         uint32_t *descriptors, const rk_page_entry *const *tables,
                         const rk_verify_params *lane_params, rk_kv_layer layer, void *stream);
 /* No counterpart in the reference. rk_attention_decode with a score shape (rk_score_shape): only the pages with a token
- * that the row sees are read. Plan, scratch and status word as for rk_attention_decode. Here and below, the key and value
+ * that the row sees are read. Plan, scratch and status word as for rk_attention_decode. Of all
+ * three decode calls, queries, partials, fp32 rows and prefix descriptors start on 16-byte boundaries, output, statistics,
+ * descriptors and tables on 8-byte ones; others are refused. Here and below, the key and value
  * rows of tokens that a row sees have to be finite; what the others hold does not matter. A query row with an element that
  * is no number comes out as zeros, with a shape and without, as from the other entries. */
 int rk_attention_decode_shaped(const void *window, const rk_decode_plan *plan, uint32_t format, const void *queries,

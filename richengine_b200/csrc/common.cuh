@@ -20,6 +20,11 @@ constexpr int kRefused = -4;     // capacity refusal (allocator, tier)
 constexpr int kTimeout = -5;     // a bounded device wait ran out
 
 void set_error(const char *text);
+
+// Whether every address (a null one too) is a multiple of `bytes`.
+template <typename... Pointers> inline bool aligned_to(uintptr_t bytes, const Pointers *...pointers) {
+  return ((reinterpret_cast<uintptr_t>(pointers) | ...) & (bytes - 1)) == 0;
+}
 int cuda_status(cudaError_t error, const char *what);
 
 // Pages of one host-tier batch, carried in a kernel's arguments: nothing is copied or allocated per transfer.

@@ -1963,6 +1963,12 @@ static int launch_decode(uint32_t format, uint32_t ctas, cudaStream_t s, const W
   }
 }
 
+// What the kernels' words need: queries, partials and fp32 rows move 16 bytes at a time, the others 8.
+static bool decode_aligned(const void *queries, const void *output, const float *output_f32, const float *partials, const float *statistics,
+                           const uint32_t *descriptors, const rk_page_entry *const *tables) {
+  return aligned_to(16, queries, output_f32, partials) && aligned_to(8, output, statistics, descriptors, tables);
+}
+
 int rk::launch_decode_suffix(uint32_t format, const rk_decode_plan &plan, cudaStream_t stream, const Window *window, const void *queries,
                              float *partials, float *statistics, uint32_t *descriptors, const rk_page_entry *const *tables,
                              const rk_verify_params *lane_params, rk_kv_layer layer, const ShapeArgs &shape, const uint32_t *lane_groups,
@@ -2030,6 +2036,10 @@ int rk_attention_decode(const void *window, const rk_decode_plan *plan, uint32_t
     set_error("rk_attention_decode: invalid arguments");
     return kInvalid;
   }
+  if (!decode_aligned(queries, output, output_f32, partials, statistics, descriptors, tables)) {
+    set_error("rk_attention_decode: queries, partials and fp32 rows start on 16-byte boundaries, the rest on 8-byte ones");
+    return kInvalid;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int st = configure_decode_kernel()) return st;
   DecodeArgs args{static_cast<const uint16_t *>(queries), partials, statistics, descriptors, tables, lane_params, layer, w->base, plan->lanes,
@@ -2049,6 +2059,10 @@ int rk_attention_decode_shaped(const void *window, const rk_decode_plan *plan, u
   if (!w || !plan || !queries || !output || !partials || !statistics || !descriptors || !tables || !lane_params ||
       !layer.extent_pages || format < RK_FORMAT_INT8 || format > RK_FORMAT_FP8E4M3 || !shape || !shape_arguments(shape, shape_args)) {
     set_error("rk_attention_decode_shaped: invalid arguments");
+    return kInvalid;
+  }
+  if (!decode_aligned(queries, output, output_f32, partials, statistics, descriptors, tables)) {
+    set_error("rk_attention_decode_shaped: queries, partials and fp32 rows start on 16-byte boundaries, the rest on 8-byte ones");
     return kInvalid;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -172,6 +172,10 @@ extern "C" int rk_attention_verify_split_shaped(const void *window, uint32_t for
     set_error("rk_attention_verify_split_shaped: invalid arguments");
     return kInvalid;
   }
+  if (!aligned_to(16, queries, partials) || !aligned_to(8, statistics, tables)) {
+    set_error("rk_attention_verify_split_shaped: queries and partials start on 16-byte boundaries, statistics and tables on 8-byte ones");
+    return kInvalid;
+  }
   const auto *w = static_cast<const Window *>(window);
   VerifyPlacement::Args args{{static_cast<const uint16_t *>(queries), partials, statistics, layer, w->base, status, kSpinLimit, shape_args},
                              tables, lane_params, lanes, grid_splits, row_capacity};
@@ -188,6 +192,10 @@ extern "C" int rk_attention_prefill_split_shaped(const void *window, uint32_t fo
   if (int st = common_arguments("rk_attention_prefill_split_shaped", window, format, kv_heads, query_heads, head_dim, shape, shape_args)) return st;
   if (!queries || !partials || !statistics || !table || !params || !status || !rk_prefill_contract_valid(params)) {
     set_error("rk_attention_prefill_split_shaped: invalid arguments");
+    return kInvalid;
+  }
+  if (!aligned_to(16, queries, partials) || !aligned_to(8, statistics, table)) {
+    set_error("rk_attention_prefill_split_shaped: queries and partials start on 16-byte boundaries, statistics and tables on 8-byte ones");
     return kInvalid;
   }
   const auto *w = static_cast<const Window *>(window);

@@ -369,6 +369,11 @@ int rk_attention_decode_shared(const void *window, const rk_shared_plan *plan, u
     set_error("rk_attention_decode_shared: invalid arguments");
     return kInvalid;
   }
+  if (!aligned_to(16, queries, output_f32, buffers->partials, buffers->prefix_partials, buffers->prefix_descriptors) ||
+      !aligned_to(8, output, buffers->statistics, buffers->descriptors, buffers->prefix_statistics, tables)) {
+    set_error("rk_attention_decode_shared: queries, partials, fp32 rows and prefix descriptors start on 16-byte boundaries, the rest on 8-byte ones");
+    return kInvalid;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const uint32_t lanes = plan->decode.lanes;
   const PrefixArgs args{{static_cast<const uint16_t *>(queries), buffers->prefix_partials, buffers->prefix_statistics, layer, w->base,

@@ -78,6 +78,47 @@ def test_shared_plan_and_missing_arguments():
         assert b"rk_attention_decode_shared" in library.rk_last_error()
 
 
+# What each entry moves 16 (8) bytes at a time, by the position of its argument; a window of zeros that nothing looks at.
+WINDOW = C.create_string_buffer(8192)
+
+
+def attention_calls():
+    library, layer, shape = lib.load(), lib.KvLayer(128, 0), lib.ScoreShape(0.0, 9, 0, 0, None)
+    plan, prefill = lib.DecodePlan(4, 148, 152), lib.PrefillParams(0, 8, 32, 1, layer, 1, 0.0)
+    shared = lib.SharedPlan(plan, 148)
+    return {
+        "rk_attention_decode": (library.rk_attention_decode, [WINDOW, C.byref(plan), abi.INT4, 32, 32, 32, 32, 32, 32, 32, 32, layer, None],
+                                (3, 5, 6), (4, 7, 8, 9)),
+        "rk_attention_decode_shaped": (library.rk_attention_decode_shaped, [WINDOW, C.byref(plan), abi.INT4, 32, 32, 32, 32, 32, 32, 32, 32, layer,
+                                                                            C.byref(shape), None], (3, 5, 6), (4, 7, 8, 9)),
+        "rk_attention_verify_split_shaped": (library.rk_attention_verify_split_shaped, [WINDOW, abi.INT4, 4, 24, 256, 1, 8, 1, 32, 32, 32, 32, 32, layer,
+                                                                                        C.byref(shape), 32, None], (8, 9), (10, 11)),
+        "rk_attention_prefill_split_shaped": (library.rk_attention_prefill_split_shaped, [WINDOW, abi.INT4, 4, 24, 256, 32, 32, 32, 32, C.byref(prefill),
+                                                                                          C.byref(shape), 32, None], (5, 6), (7, 8)),
+        "rk_attention_decode_shared": (library.rk_attention_decode_shared, [WINDOW, C.byref(shared), abi.INT4, 32, 32, 32, [32] * 6, 32, 32, layer, 32, 32,
+                                                                            None, None], (3, 5, (6, 0), (6, 3), (6, 5)), (4, (6, 1), (6, 2), (6, 4), 7)),
+    }
+
+
+@pytest.mark.parametrize("name", ["rk_attention_decode", "rk_attention_decode_shaped", "rk_attention_verify_split_shaped",
+                                  "rk_attention_prefill_split_shaped", "rk_attention_decode_shared"])
+def test_addresses_between_words_are_refused(name):
+    """A tensor that starts between the words its kernel moves would be a fault on the device: refused on the host, whichever it is."""
+    call, arguments, sixteens, eights = attention_calls()[name]
+    for positions, offsets in ((sixteens, (2, 4, 8)), (eights, (2, 4))):
+        for at in positions:
+            for offset in offsets:
+                changed = [list(a) if isinstance(a, list) else a for a in arguments]
+                if isinstance(at, tuple):
+                    changed[at[0]][at[1]] += offset
+                else:
+                    changed[at] += offset
+                changed = [C.byref(lib.SharedBuffers(*a)) if isinstance(a, list) else a for a in changed]
+                assert call(*changed) == lib.INVALID, (at, offset)
+                text = lib.load().rk_last_error()
+                assert text.startswith(name.encode() + b":") and b"boundaries" in text
+
+
 def test_block_sizes():
     assert C.sizeof(lib.ScoreShape) == 24 and lib.ScoreShape.slopes.offset == 16
     assert C.sizeof(lib.StepPool) == 24 and C.sizeof(lib.SharedPlan) == C.sizeof(lib.DecodePlan) + 32
