@@ -17,11 +17,12 @@ in flight.
 from __future__ import annotations
 
 import ctypes as C
+from collections import Counter
 
 import torch
 
 from . import lib, ops
-from .abi import VERIFY_CHUNK_STRIDE, Layout
+from .abi import BF16, FP8E4M3, INT4, INT8, VERIFY_CHUNK_STRIDE, Layout, pages_for
 from .storage import PageStorage
 
 
@@ -29,9 +30,28 @@ def _stream_handle(stream) -> int:
     return ops._stream(stream)
 
 
+# What a tile of a shared prefix costs, in lanes that stream the same pages: 128 rows x 64 tokens take a CTA the same time however
+# many of the rows are real (21 lanes fill them), and lanes that read the same pages by themselves find part of them in L2.
+# Measured on a B200 without a score shape: int4 loses with four lanes a group (32 groups of 8K: 176 us against 148) and wins with
+# six (20 groups of 8K: 124 against 146); int8 wins with four (215 against 234) and loses with three (211 against 184); fp8 loses
+# with four (251 against 234) and is even with five; bf16 wins with three (301 against 337) and loses with two.
+TILE_PRICE = {INT4: 4.6, INT8: 3.9, FP8E4M3: 4.2, BF16: 2.7}
+
+
+def prefix_saving(layout, groups) -> float:
+    """Bytes of pages a layer that reading shared prefixes once is worth; `groups`: (lanes, pages shared) of each."""
+    price = TILE_PRICE[layout.format]
+    tiles = (-(-lanes * 6 // 128) for lanes, _ in groups)  # six query heads a KV head
+    return sum((lanes - price * t) * pages for (lanes, pages), t in zip(groups, tiles)) * layout.bytes_per_layer_page()
+
+
 class DecodeSession:
-    kWorthBytes = 200 << 20  # pages a shared prefix has to save per layer before it is read apart
+    # What shared prefixes have to save a layer. The third kernel costs 7 us and the wider merge up to 13 more, growing with the lanes
+    # while those are few (with many, a tile has fewer splits to merge): 8 lanes of int8 over 16K, 140 MB, win (48 us to 40), 16 of
+    # bf16 over 2K, 112 MB, and 32 of int8 over 2K, 103 MB, lose (29 to 34, 32 to 40), 32 of int4 over 8K, 197 MB, win (60 to 49).
+    kWorthBytes, kWorthLaneBytes = 72 << 20, 3 << 20
     _sharing = False
+    _groups = None    # (lanes, pages shared) of each group; None: not known, or the caller has decided
 
     def __init__(self, storage: PageStorage, query_heads: int, lanes: int, ctas: int = 0):
         layout = storage.layout
@@ -66,18 +86,48 @@ class DecodeSession:
 
     def share_prefixes(self, table_pointers, verify_params, minimum_pages: int | None = None, stream=None) -> None:
         """Finds which lanes share how long a prefix; until the next call (or forget_prefixes) the device steps read every
-        shared prefix once. To be called when the batch changes: a group's pages must stay full and shared. By default a
-        group has to be able to save kWorthBytes of pages a layer, about what the extra kernel and merge cost (a B200: 25
-        against 20 us for 4 lanes over 2K int8 tokens, 52 against 61 for 32 over 8K int4, 272 against 1 364 for 256 over 32K)."""
-        if minimum_pages is None:
-            saved = max(1, self.lanes - 1) * self.layout.bytes_per_layer_page()
-            minimum_pages = max(1, -(-self.kWorthBytes // saved))
+        shared prefix once. To be called when the batch changes: a group's pages must stay full and shared. By default groups
+        are formed where a tile costs less than its lanes (TILE_PRICE) and used where together they save worth_bytes() of pages a
+        layer, which is counted anew for a layer with a sliding window; with `minimum_pages`, two lanes over that many pages are a
+        group and every layer uses it. Without a group the steps stay as they are. The call waits for the search on the GPU;
+        captured into a graph it cannot, so the default then uses whatever groups could save that much if all lanes were one."""
+        default = minimum_pages is None
         if self._shared is None:
             self._shared = ops.SharedPrefixDecode(self.layout, self.query_heads, self.lanes, self.storage.window(), self._ctas)
             self._lane_groups, self._group_pages = (torch.empty(self.lanes, dtype=torch.int32, device="cuda") for _ in range(2))
-        ops.prefix_groups(self.lanes, table_pointers, verify_params, self._lane_groups, self._group_pages, minimum_pages=minimum_pages,
-                          stream=stream)
-        self._sharing = True
+        self._sharing, self._groups, self._worth = False, None, {}
+        if stream is not None and not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(_stream_handle(stream))
+        with torch.cuda.stream(stream):
+            captured = torch.cuda.is_current_stream_capturing()
+            if default:
+                # no group of fewer pages is worth it, the largest being the whole batch
+                most = max(prefix_saving(self.layout, [(self.lanes, 1)]), 1)
+                minimum_pages = max(1, int(-(-self.worth_bytes() // most))) if captured else 1
+            ops.prefix_groups(self.lanes, table_pointers, verify_params, self._lane_groups, self._group_pages,
+                              minimum_lanes=int(TILE_PRICE[self.layout.format]) + 1 if default else 2, minimum_pages=minimum_pages)
+            if captured:
+                self._sharing = True
+                return
+            members, pages = Counter(self._lane_groups.tolist()), self._group_pages.tolist()
+            groups = [(lanes, pages[g]) for g, lanes in members.items() if g >= 0]
+            if groups and (not default or prefix_saving(self.layout, groups) >= self.worth_bytes()):
+                self._sharing, self._groups = True, groups if default else None
+            else:
+                self._lane_groups.fill_(-1)
+                self._group_pages.zero_()
+
+    def worth_bytes(self) -> int:
+        return self.kWorthBytes + min(self.lanes, 32) * self.kWorthLaneBytes
+
+    def _shares(self, shape) -> bool:
+        """Whether a layer's step reads the shared prefixes apart."""
+        if not self._sharing or self._groups is None or shape is None or not shape.window:
+            return self._sharing
+        seen = pages_for(shape.window) + pages_for(shape.sink_tokens)  # pages that a row looks at, give or take one
+        if seen not in self._worth:
+            self._worth[seen] = prefix_saving(self.layout, [(lanes, min(pages, seen)) for lanes, pages in self._groups]) >= self.worth_bytes()
+        return self._worth[seen]
 
     def forget_prefixes(self) -> None:
         """The device steps go back to one stream of pages per lane."""
@@ -90,7 +140,7 @@ class DecodeSession:
             self._shared.status(stream)
 
     def _attend(self, layer: int, table_pointers, verify_params, stream, shape) -> None:
-        if self._sharing:
+        if self._shares(shape):
             self._shared.run(self.queries, self.output, table_pointers, verify_params, self.layers[layer], self._lane_groups,
                              self._group_pages, stream=stream, shape=shape)
             self.kernel_launches += 3
@@ -112,8 +162,8 @@ class DecodeSession:
 
     def step_host(self, layer: int, q_host, k_host, v_host, out_host, table_pointers, chunk_params, verify_params,
                   stream=None) -> None:
-        """q_host [lanes][query_heads][D], k_host / v_host [lanes][kv_heads][D], out_host like q_host:
-        pinned bf16 host tensors. One C call (rk_session_step_host: uploads, append, attention, download, all
+        """The step lane by lane, also while prefixes are shared. q_host [lanes][query_heads][D], k_host / v_host
+        [lanes][kv_heads][D], out_host like q_host: pinned bf16 host tensors. One C call (rk_session_step_host: uploads, append, attention, download, all
         asynchronous); out_host is valid after finish_host() and a synchronise of the stream. The host tensors must
         stay unchanged until then."""
         lib.check(self._lib.rk_session_step_host(self._host_session(), layer, q_host.data_ptr(), k_host.data_ptr(),

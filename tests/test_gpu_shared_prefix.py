@@ -346,3 +346,84 @@ def test_a_query_row_that_is_no_number_comes_out_as_zeros(fmt, shape):
         check_rows(got32[lane, :, 0], None, want, bound + 2.0 ** -20 * np.abs(want).max(), f"lane {lane}")
     s.check(got16, got32, shape, lanes=[l for l in range(s.lanes) if l not in (grouped, loose)])
     s.batch.close()
+
+
+def session_of(s):
+    """A session over a Shared batch, its queries in place; and a step's rows and launches."""
+    from richengine_b200.session import DecodeSession
+    session = DecodeSession(s.batch.storage, 24, s.lanes)
+    session.queries.copy_(dev(s.queries).view(torch.bfloat16))
+    params = s.batch.params(s.committed)
+
+    def attend(shape=None):
+        before = session.kernel_launches
+        session.output.zero_()
+        session.attend_device(0, s.batch.pointers, params, shape=shape_of(shape) if shape else None)
+        return host16(session.output), session.kernel_launches - before
+
+    return session, params, attend
+
+
+def check16(s, got16, lanes, shape=None):
+    for lane in lanes:
+        want, bound = s.batch.attend(lane, s.committed[lane], s.queries[lane, :, 0], shape)
+        got = (got16[lane, :, 0].astype(np.uint32) << 16).view(np.float32)
+        assert (np.abs(got - want) <= bound + 2.0 ** -20 * np.abs(want).max() + np.abs(want) * 2.0 ** -8 + bound * 2.0 ** -8).all(), lane
+
+
+@pytest.mark.parametrize("fmt", [INT4, BF16])
+def test_a_session_shares_only_what_is_worth_it(fmt):
+    """By default: a pair in a large batch is not read apart, however the pair would look if all lanes shared its pages; nor is a batch
+    without a group, whichever way it is asked; the step is then the plain one. A group that saves enough is, but not in a layer
+    whose window leaves little of it."""
+    pair = Shared(fmt, [(110, 2)], 62, suffix=20)
+    session, params, attend = session_of(pair)
+    session.share_prefixes(pair.batch.pointers, params)
+    got16, launches = attend()
+    assert launches == 2 and int(session._group_pages.max()) == 0 and int(session._lane_groups.max()) == -1
+    check16(pair, got16, sorted({pair.member.index(0), 0, 63}))
+    session.share_prefixes(pair.batch.pointers, params, minimum_pages=100)  # a caller's own threshold holds
+    shared16, launches = attend()
+    assert launches == 3 and int(session._group_pages.max()) == 110
+    check16(pair, shared16, sorted({pair.member.index(0), 0, 63}))
+    session.share_prefixes(pair.batch.pointers, params, minimum_pages=111)
+    again16, launches = attend()
+    assert launches == 2 and np.array_equal(again16, got16)
+    session.close()
+    pair.batch.close()
+
+    many = Shared(fmt, [(40, 24)], 3, suffix=20)
+    session, params, attend = session_of(many)
+    session.kWorthLaneBytes, session.kWorthBytes = 0, 40 * many.batch.layout.bytes_per_layer_page()  # a threshold that small pools reach
+    session.share_prefixes(many.batch.pointers, params)
+    for shape, expected in ((None, 3), ((9.0, 0, 0, None), 3), ((0.0, 32 * 39, 0, None), 3), ((0.0, 20, 0, None), 2), ((0.0, 20, 32 * 39, None), 3)):
+        got16, launches = attend(shape)
+        assert launches == expected, shape
+        check16(many, got16, (0, 13, 26), shape)
+    session.forget_prefixes()
+    assert attend()[1] == 2
+    session.close()
+    many.batch.close()
+
+
+def test_a_captured_search_decides_on_the_gpu():
+    """share_prefixes inside a capture cannot wait for its result: the groups of each replay are used as they are found."""
+    s = Shared(INT4, [(6, 9)], 2, suffix=20)
+    session, params, attend = session_of(s)
+    session.kWorthLaneBytes, session.kWorthBytes = 0, 6 * s.batch.layout.bytes_per_layer_page()
+    session.share_prefixes(s.batch.pointers, params)
+    eager16, launches = attend()
+    assert launches == 3
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        session.share_prefixes(s.batch.pointers, params, stream=stream)
+        session.attend_device(0, s.batch.pointers, params, stream=stream)
+    session.output.zero_()
+    session._group_pages.zero_()
+    graph.replay()
+    assert np.array_equal(host16(session.output), eager16) and int(session._group_pages.max()) == 6
+    del graph
+    session.close()
+    s.batch.close()
