@@ -163,6 +163,14 @@ int rk_attention_verify_probe_timeout(const void *window, uint32_t format, uint3
                                       const rk_page_entry *const *tables, const rk_verify_params *lane_params,
                                       rk_kv_layer layer, uint32_t *status, uint32_t spin_limit,
                                       uint32_t withheld_groups, void *stream);
+/* The same for the row-tile kernel of the shaped entries: rk_attention_verify_split_shaped on at most `ctas` CTAs whose TMA
+ * warp streams nothing more from the last `withheld_groups` groups of its first item on. */
+int rk_attention_shaped_probe_timeout(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,
+                                      uint32_t head_dim, uint32_t lanes, uint32_t row_capacity, uint32_t grid_splits,
+                                      const void *queries, float *partials, float *statistics,
+                                      const rk_page_entry *const *tables, const rk_verify_params *lane_params,
+                                      rk_kv_layer layer, const rk_score_shape *shape, uint32_t *status, uint32_t ctas,
+                                      uint32_t spin_limit, uint32_t withheld_groups, void *stream);
 int rk_attention_decode(const void *window, const rk_decode_plan *plan, uint32_t format, const void *queries,
                         void *output, float *output_f32, float *partials, float *statistics,
                         uint32_t *descriptors, const rk_page_entry *const *tables,

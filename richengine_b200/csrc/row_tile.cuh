@@ -75,6 +75,7 @@ struct RowTileArgs {
   uint32_t *status;
   uint32_t spin_limit;
   ShapeArgs shape;
+  uint32_t withheld_groups = 0; // timeout probe only: from an item's last groups on, nothing more is streamed
 };
 
 // ---- a softmax thread's scores --------------------------------------------------------------------------------------------
@@ -470,7 +471,10 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
       const uint64_t region_base = args.layer.offset + extent_pages * (kind == 0 ? 0ull : kind == 2 ? uint64_t(data_bytes)
                                                                         : kind == 1 ? uint64_t(data_bytes) + scale_bytes : 2ull * data_bytes + scale_bytes);
       const uint32_t page_stride = kind < 2 ? data_bytes : scale_bytes;
-      uint32_t done = 0;
+      // A wait that gave up (here or elsewhere) ends the streaming: a stage may then still be waiting for its last copy, and a
+      // second one on the same barrier would leave its phases out of step with the wait for the copies below.
+      uint32_t done = 0, issued = 0;
+      bool stopped = false;
       for (uint32_t k = 0; k < mine; ++k) {
         const RowItem &item = item_of(k);
         const uint32_t begin = item.ordinal_begin, end = item.ordinal_end, groups = (end - begin + 1) / 2;
@@ -478,11 +482,14 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
         const rk_page_entry *table = item.table;
         const uint64_t tensor_base = region_base + item.head * (kind < 2 ? kSlab : 128u);
         rk_page_entry next = lane < 8 && begin + local < end ? table[list.page(begin + local)] : 0;
-        for (uint32_t g = 0; g < groups; ++g) {
+        for (uint32_t g = 0; g < groups && !stopped; ++g) {
           const uint32_t n = done + g, r = n % kRawStages, first = begin + 2 * g, group_pages = min(2u, end - first);
           const rk_page_entry entry = next;
           if (lane < 8 && first + 2 + local < end) next = table[list.page(first + 2 + local)];
           if (n >= kRawStages) barrier_wait(&sh.raw_free[r], n / kRawStages - 1, error);
+          stopped = __any_sync(0xffffffffu, *error != 0) || g + args.withheld_groups >= groups;
+          if (stopped) break;
+          issued = n + 1;
           const uint32_t full = smem_u32(&sh.raw_full[r]), stage = raw_tile + r * kRawStageBytes;
           if (lane == 0) barrier_expect(full, group_pages * (2 * kSlab + (Kind::kScales ? 256 : 0)));
           __syncwarp();
@@ -496,7 +503,7 @@ row_tile_kernel(const __grid_constant__ CUtensorMap head_map, const __grid_const
       }
       // every copy this warp started has landed before the CTA may leave (also after a failed wait)
       if (lane == 0)
-        for (uint32_t n = done > kRawStages ? done - kRawStages : 0; n < done; ++n) {
+        for (uint32_t n = issued > kRawStages ? issued - kRawStages : 0; n < issued; ++n) {
           const uint32_t bar = smem_u32(&sh.raw_full[n % kRawStages]), parity = (n / kRawStages) & 1u;
           for (uint32_t i = 0; i < kSpinLimit && !barrier_try(bar, parity); ++i) __nanosleep(64);
         }

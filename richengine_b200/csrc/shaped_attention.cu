@@ -156,32 +156,60 @@ int tile::persistent_ctas(uint64_t items, uint32_t &ctas) {
 
 using namespace rk;
 
+static int verify_split_shaped(const char *what, const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,
+                               uint32_t head_dim, uint32_t lanes, uint32_t row_capacity, uint32_t grid_splits, const void *queries,
+                               float *partials, float *statistics, const rk_page_entry *const *tables, const rk_verify_params *lane_params,
+                               rk_kv_layer layer, const rk_score_shape *shape, uint32_t *status, uint32_t most_ctas, uint32_t spin_limit,
+                               uint32_t withheld_groups, void *stream) {
+  ShapeArgs shape_args;
+  if (int st = common_arguments(what, window, format, kv_heads, query_heads, head_dim, shape, shape_args)) return st;
+  if (row_capacity != 8 && row_capacity != 16) {
+    set_error((std::string(what) + ": row capacity 8 or 16; one row takes rk_attention_decode_shaped").c_str());
+    return kUnsupported;
+  }
+  if (!lanes || lanes > 65535 || !grid_splits || grid_splits > RK_VERIFY_MAX_SPLITS || !queries || !partials || !statistics || !tables || !lane_params ||
+      !layer.extent_pages || !status) {
+    set_error((std::string(what) + ": invalid arguments").c_str());
+    return kInvalid;
+  }
+  if (!aligned_to(16, queries, partials) || !aligned_to(8, statistics, tables)) {
+    set_error((std::string(what) + ": queries and partials start on 16-byte boundaries, statistics and tables on 8-byte ones").c_str());
+    return kInvalid;
+  }
+  const auto *w = static_cast<const Window *>(window);
+  VerifyPlacement::Args args{{static_cast<const uint16_t *>(queries), partials, statistics, layer, w->base, status, spin_limit, shape_args,
+                              withheld_groups},
+                             tables, lane_params, lanes, grid_splits, row_capacity};
+  uint32_t ctas = 0;
+  if (int st = persistent_ctas(uint64_t(kHeads) * grid_splits * lanes, ctas)) return st;
+  return launch_row_tile<VerifyPlacement>(format, w, ctas < most_ctas ? ctas : most_ctas, args, static_cast<cudaStream_t>(stream));
+}
+
 extern "C" int rk_attention_verify_split_shaped(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,
                                                 uint32_t head_dim, uint32_t lanes, uint32_t row_capacity, uint32_t grid_splits,
                                                 const void *queries, float *partials, float *statistics,
                                                 const rk_page_entry *const *tables, const rk_verify_params *lane_params,
                                                 rk_kv_layer layer, const rk_score_shape *shape, uint32_t *status, void *stream) {
-  ShapeArgs shape_args;
-  if (int st = common_arguments("rk_attention_verify_split_shaped", window, format, kv_heads, query_heads, head_dim, shape, shape_args)) return st;
-  if (row_capacity != 8 && row_capacity != 16) {
-    set_error("rk_attention_verify_split_shaped: row capacity 8 or 16; one row takes rk_attention_decode_shaped");
-    return kUnsupported;
-  }
-  if (!lanes || lanes > 65535 || !grid_splits || grid_splits > RK_VERIFY_MAX_SPLITS || !queries || !partials || !statistics || !tables || !lane_params ||
-      !layer.extent_pages || !status) {
-    set_error("rk_attention_verify_split_shaped: invalid arguments");
+  return verify_split_shaped("rk_attention_verify_split_shaped", window, format, kv_heads, query_heads, head_dim, lanes, row_capacity, grid_splits,
+                             queries, partials, statistics, tables, lane_params, layer, shape, status, ~0u, kSpinLimit, 0, stream);
+}
+
+// Test hook of the row-tile kernel's timeout path: the same launch on at most `ctas` CTAs with waits that give up after
+// `spin_limit` polls and a TMA warp that streams nothing more from the last `withheld_groups` 64-token groups of its first item
+// on. Every later wait of the CTA gives up at once, the copies under way land, tensor memory is released, `status` turns
+// non-zero and the kernel returns; nothing faults and no wait is unbounded. The step's output is invalid.
+extern "C" int rk_attention_shaped_probe_timeout(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,
+                                                 uint32_t head_dim, uint32_t lanes, uint32_t row_capacity, uint32_t grid_splits,
+                                                 const void *queries, float *partials, float *statistics,
+                                                 const rk_page_entry *const *tables, const rk_verify_params *lane_params,
+                                                 rk_kv_layer layer, const rk_score_shape *shape, uint32_t *status, uint32_t ctas,
+                                                 uint32_t spin_limit, uint32_t withheld_groups, void *stream) {
+  if (!ctas || !spin_limit || spin_limit > kSpinLimit || withheld_groups > rk_pages_for(RK_MAX_PHYSICAL_TOKENS)) {
+    set_error("rk_attention_shaped_probe_timeout: CTAs, spin limit or withheld groups out of range");
     return kInvalid;
   }
-  if (!aligned_to(16, queries, partials) || !aligned_to(8, statistics, tables)) {
-    set_error("rk_attention_verify_split_shaped: queries and partials start on 16-byte boundaries, statistics and tables on 8-byte ones");
-    return kInvalid;
-  }
-  const auto *w = static_cast<const Window *>(window);
-  VerifyPlacement::Args args{{static_cast<const uint16_t *>(queries), partials, statistics, layer, w->base, status, kSpinLimit, shape_args},
-                             tables, lane_params, lanes, grid_splits, row_capacity};
-  uint32_t ctas = 0;
-  if (int st = persistent_ctas(uint64_t(kHeads) * grid_splits * lanes, ctas)) return st;
-  return launch_row_tile<VerifyPlacement>(format, w, ctas, args, static_cast<cudaStream_t>(stream));
+  return verify_split_shaped("rk_attention_shaped_probe_timeout", window, format, kv_heads, query_heads, head_dim, lanes, row_capacity, grid_splits,
+                             queries, partials, statistics, tables, lane_params, layer, shape, status, ctas, spin_limit, withheld_groups, stream);
 }
 
 extern "C" int rk_attention_prefill_split_shaped(const void *window, uint32_t format, uint32_t kv_heads, uint32_t query_heads,

@@ -104,6 +104,7 @@ SIGNATURES = {
     "rk_attention_verify_split": (i32, [u32, u32, u32, u32, u32, u32, u32, vp, vp, vp, vp, vp, vp, KvLayer, vp]),
     "rk_attention_verify_split_tc": (i32, [vp, u32, u32, u32, u32, u32, u32, u32, vp, vp, vp, vp, vp, vp, KvLayer, vp, vp]),
     "rk_attention_verify_split_shaped": (i32, [vp, u32, u32, u32, u32, u32, u32, u32, vp, vp, vp, vp, vp, KvLayer, C.POINTER(ScoreShape), vp, vp]),
+    "rk_attention_shaped_probe_timeout": (i32, [vp, u32, u32, u32, u32, u32, u32, u32, vp, vp, vp, vp, vp, KvLayer, C.POINTER(ScoreShape), vp, u32, u32, u32, vp]),
     "rk_attention_prefill_split_shaped": (i32, [vp, u32, u32, u32, u32, vp, vp, vp, vp, C.POINTER(PrefillParams), C.POINTER(ScoreShape), vp, vp]),
     "rk_attention_verify_probe_timeout": (i32, [vp, u32, u32, u32, u32, u32, u32, u32, vp, vp, vp, vp, vp, KvLayer, vp, u32, u32, vp]),
     "rk_attention_verify_reduce": (i32, [u32, u32, u32, u32, u32, vp, vp, vp, vp, vp, vp]),

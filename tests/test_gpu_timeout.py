@@ -168,3 +168,39 @@ def test_exchange_wait_for_a_peer_runs_out_is_reported_and_recovers():
     _, want32 = run_verify_attention_oracle(s, q, 1, 1)
     assert_attention_close(out32.cpu().numpy(), want32, host_u16(out), "the complete step after a timeout")
     exchange.close(); s.close()
+
+
+@pytest.mark.parametrize("fmt", [INT4, INT8, FP8E4M3, BF16])
+@pytest.mark.parametrize("ctas,spin_limit,withheld", [(1, SPIN_LIMIT, 1), (2, SPIN_LIMIT, 2), (148, SPIN_LIMIT, 1), (3, 1, 1)])
+def test_row_tile_wait_runs_out_is_reported_and_recovers(fmt, ctas, spin_limit, withheld):
+    """Few CTAs, so that a block goes on through more items than it plans at a time after the wait that ran out; many; and waits that
+    give up at the second poll."""
+    library = lib.load()
+    s, q = prepared([700, 500, 90, 333], fmt, seed=37)
+    rows, splits = 8, 2
+    committed = [c - rows + 1 for c in s.contexts]
+    params, slot = verify_params(s, rows, rows, splits, committed=committed)
+    d_params, dq = struct_to_device(params), dev(q)
+    partials = torch.zeros(s.lanes * 4 * slot * rows * 6 * 256, dtype=torch.float32, device="cuda")
+    stats = torch.zeros(s.lanes * 4 * slot * rows * 6 * 2, dtype=torch.float32, device="cuda")
+    runner = ops.VerifyWindowAttention(s.layout, 24, s.storage.window())
+    layer, shape = s.storage.layers()[0], ops.ScoreShape()
+    status = library.rk_attention_shaped_probe_timeout(
+        runner._window, fmt, 4, 24, 256, s.lanes, rows, slot, dq.data_ptr(), partials.data_ptr(), stats.data_ptr(),
+        s.table_pointers.data_ptr(), d_params.data_ptr(), layer, shape.block(24), runner.status_word.data_ptr(), ctas, spin_limit, withheld,
+        torch.cuda.current_stream().cuda_stream)
+    assert status == lib.OK, library.rk_last_error()
+    torch.cuda.synchronize()  # the kernel came back and released its tensor memory
+    with pytest.raises(lib.RichKvError) as caught:
+        runner.check()
+    assert caught.value.status == lib.TIMEOUT
+    runner.status_word.zero_()
+    # the next ordinary launch on the same buffers is correct
+    out, out32 = torch.zeros_like(dq), torch.zeros(dq.shape, dtype=torch.float32, device="cuda")
+    runner.split(s.lanes, rows, slot, dq, partials, stats, s.table_pointers, None, d_params, layer, shape=shape)
+    ops.attention_verify_reduce(s.layout, 24, s.lanes, rows, partials, stats, out, d_params, output_f32=out32)
+    runner.check()
+    _, want32 = run_verify_attention_oracle(s, q, rows, rows, committed=committed)
+    assert_attention_close(out32.cpu().numpy(), want32, host_u16(out), "row tiles after a timeout")
+    runner.close()
+    s.close()
