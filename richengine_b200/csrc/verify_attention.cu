@@ -223,8 +223,9 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
     // table entries travel one group ahead of their use (copies) and of their L2 request (prefetch)
     rk_page_entry next = lane < 8 && page_begin + local < page_end ? table[page_begin + local] : 0;
     rk_page_entry next_ahead = prefetcher && page_begin + 2 * kPrefetchGroups + local < page_end ? table[page_begin + 2 * kPrefetchGroups + local] : 0;
-    const uint32_t issued = groups - min(groups, args.withheld_groups); // all of them, except under the timeout probe
-    for (uint32_t g = 0; g < issued; ++g) {
+    const uint32_t streamed = groups - min(groups, args.withheld_groups); // all of them, except under the timeout probe
+    uint32_t issued = 0;
+    for (uint32_t g = 0; g < streamed; ++g) {
       const uint32_t r = g % kRawStages;
       const uint32_t first = page_begin + 2 * g, group_pages = min(2u, page_end - first);
       const rk_page_entry entry = next, entry_ahead = next_ahead;
@@ -232,6 +233,10 @@ window_attention_kernel(const __grid_constant__ CUtensorMap head_map, VerifyArgs
       if (lane < 8 && first + 2 + local < page_end) next = table[first + 2 + local];
       if (prefetcher && ahead + 2 < page_end) next_ahead = table[ahead + 2];
       if (g >= kRawStages) barrier_wait(&ctl.raw_free[r], g / kRawStages - 1, error); // the stage's last readers
+      // A wait that gave up, anywhere in the CTA, ends the streaming: the stage may still be waiting for its last copy, and a second
+      // one on its barrier would leave the phases out of step with the wait for the copies below.
+      if (__any_sync(0xffffffffu, *error != 0)) break;
+      issued = g + 1;
       const uint32_t full = smem_u32(&ctl.raw_full[r]), stage = raw_tile + r * kRawStageBytes;
       if (lane == 0) barrier_expect(full, group_pages * (2 * kSlab + (Kind::kScales ? 256 : 0)));
       __syncwarp();
