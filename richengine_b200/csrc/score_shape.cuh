@@ -55,15 +55,20 @@ __device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
 }
 
 // cap * tanh(s / cap) for N scores, tanh(u) = 1 - 2 / (e^2u + 1). The hardware's own tanh (2^-11) would move a score of 30
-// by 0.015; this form has an absolute error of about cap * 2^-22. Four scores share one reciprocal (1/a = b c d / (a b c d)):
-// five special-function operations for four scores instead of eight, in the softmax warps of a 16-row window, which are
-// short of that unit (four lanes over 32K int4 tokens: 115 us, and 121 with a reciprocal each; 86 without a cap). e^2u stops at 2^30, where the quotient is under half a step of one, so that four of them stay finite.
-// Caps up to 256 take this form: its error is under 2^-13 on a score, where the weights are rounded to 2^-11. Beyond, scores
-// are small against the cap and the difference from one loses them: below |u| = 1/4 the odd series u (1 - u^2/3 + 2u^4/15 -
-// 17u^6/315 + 62u^8/2835), whose next term is under 10^-8 there, takes over, and the result is good to about 10^-6 of itself.
+// by 0.015. Four scores share one reciprocal (1/a = b c d / (a b c d)): five special-function operations for four scores instead
+// of eight; four lanes over 32K int4 tokens: 115 us, and 121 with a reciprocal each (86 without a cap: what the cap adds is the
+// length of a group's chain, the special-function unit is a third busy). e^2u stops at 2^30, where the quotient is under half a
+// step of one, so that four of them stay finite.
+// Error of this form, in units of cap * 2^-23, from the sum of its roundings with q = 1 / (e^2u + 1) <= 1: the exponent's six
+// (its scale and products) 2 * 0.67, ex2 (2^-22) and the sum with one 2 * (0.5 + 0.5), the reciprocal (2^-23) and four products
+// 2 * 3, the last multiply-add 0.5: under 10, cap * 2^-19.7 (the worst of 16 million scores was cap * 2^-21.0 in a replay with
+// exact ex2 and rcp). Caps up to 64 take it: under 2^-13 on a score, a quarter of what rounding the weights to 11 bits allows.
+// Beyond, scores are small against the cap and the difference from one loses them: below |u| = 1/4 the odd series u (1 - u^2/3 +
+// 2u^4/15 - 17u^6/315 + 62u^8/2835), whose next term is under 10^-8 there, takes over, and the result is good to about 10^-6 of
+// itself (the four lanes: 123 us with a cap of 100, 110 with one of 50).
 // A score that is no number stays one, and takes the three that share its reciprocal with it: callers pass scores of one query
 // row, s[4i] .. s[4i + 3], and give tokens that the row does not see (their keys may hold anything) a finite score beforehand.
-constexpr float kDirectCap = 256.0f * 1.4426950408889634f;
+constexpr float kDirectCap = 64.0f * 1.4426950408889634f;
 __device__ __forceinline__ float exp2_special(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

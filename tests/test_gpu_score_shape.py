@@ -330,3 +330,53 @@ class Lane:
     def __init__(self, batch, lane):
         self.layout, self.layer, self.storage = batch.layout, batch.layer, batch.storage
         self.pages, self.tables = [batch.pages[lane]], [batch.tables[lane]]
+
+
+@pytest.mark.parametrize("fmt", [INT4, BF16])
+@pytest.mark.parametrize("cap", [1.0, 63.0, 64.0, 65.0, 255.0, 256.0, 257.0])
+@pytest.mark.parametrize("reach", [0.05, 3.0])
+def test_caps_on_both_sides_of_the_switch(fmt, cap, reach):
+    """Scores far below the cap and past it, of both signs, at caps around the one where the form of the tanh changes. The form for the
+    smaller caps is off by at most cap * 2^-19.7 on a score, which moves a weight by that and the row by twice that of its largest
+    value; the other by 10^-6 of the score, which the bound of every row allows."""
+    contexts = [300, 64]
+    batch, q = prepared(fmt, contexts, 8)
+    scale = 2.0 ** round(np.log2(reach * cap / 48))  # the largest of a row's scores q.k is near 48
+    shape = (cap, 0, 0, None)
+    for lane, context in enumerate(contexts):
+        largest = max(np.abs(v).max() for v in [batch.rows(lane, range(context + 1))[1]])
+        slack = 2 * cap * 2.0 ** -19.7 * largest if cap <= 64 else 0.0
+        params = batch.params(contexts, score_scale=scale)
+        got16, got32 = decode(batch, contexts, q, shape_of(shape), params=params)
+        want, bound = batch.attend(lane, context, q[lane, :, 0], shape, scale)
+        check_rows(got32[lane, :, 0], got16[lane, :, 0], want, bound + slack, f"decode, lane {lane}")
+        plain_params = batch.params
+        batch.params = lambda *arguments: plain_params(*arguments, score_scale=scale)
+        got16, got32 = verify(batch, contexts, 8, 8, q, shape_of(shape), 2)
+        batch.params = plain_params
+        for r in (0, 7):
+            want, bound = batch.attend(lane, context + r, q[lane, :, r], shape, scale)
+            check_rows(got32[lane, :, r], got16[lane, :, r], want, bound + slack, f"verify, lane {lane}, row {r}")
+    batch.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_negative_slopes(fmt):
+    """Slopes of either sign, the far tokens favoured by half of the heads."""
+    slopes = [(-1.0) ** h * 2.0 ** (-4 - h / 8) for h in range(24)]
+    contexts = [500, 31, 1055]
+    batch, q = prepared(fmt, contexts, 8)
+    for shape in ((0.0, 0, 0, slopes), (20.0, 300, 40, slopes)):
+        block = shape_of(shape)
+        got16, got32 = decode(batch, contexts, q, block)
+        window16, window32 = verify(batch, contexts, 8, 8, q, block, 3)
+        chunk16, chunk32 = prefill(Lane(batch, 0), contexts[0], 8, q[0], block, 1)
+        for lane, context in enumerate(contexts):
+            want, bound = batch.attend(lane, context, q[lane, :, 0], shape)
+            check_rows(got32[lane, :, 0], got16[lane, :, 0], want, bound, f"decode, lane {lane}")
+            for r in (0, 7):
+                want, bound = batch.attend(lane, context + r, q[lane, :, r], shape)
+                check_rows(window32[lane, :, r], window16[lane, :, r], want, bound, f"verify, lane {lane}, row {r}")
+                if lane == 0:
+                    check_rows(chunk32[:, r], chunk16[:, r], want, bound, f"prefill, row {r}")
+    batch.close()
