@@ -108,7 +108,8 @@ typedef struct rk_score_shape {
 } rk_score_shape;
 
 /* Where page ids lie (rk_storage_step_pool): page id i is page i % extent_pages of the extent at
- * base + i / extent_pages * extent_stride. */
+ * base + i / extent_pages * extent_stride. All page_count of them have to lie in the window that the attention calls are
+ * given: an id below page_count is not checked further. */
 typedef struct rk_step_pool {
   uint64_t base, extent_stride;
   uint32_t extent_pages, page_count;

@@ -18,7 +18,8 @@
 // and shared memory about 2 100 (1 450 wavefronts of loads and stores, half of them scales that every row's thread reads, 128
 // of the copies in, 512 of the matrix unit's operand reads). Work left out in a copy: without the softmax the 256-lane prefix
 // takes 188 us instead of 222, without the expansion 205, without either 157, without the scales' reads 205: several limits
-// lie close together. What a shape adds to the softmax shows in full (a cap 26 us of 85, slopes 20 % of a prefill chunk).
+// lie close together. What a shape adds to the softmax shows in full (a cap 26 us of 85, slopes 20 % of a prefill chunk), for the rows
+// that do not exist too: the softmax warps work on all 128, of which a 16-row window fills 96 and an 8-row one 48.
 // Sixteen softmax warps because eight were latency bound (a group's chain of load, maximum,
 // weights and store is shorter with 16 scores a thread than with 32); two teams of eight that alternate between groups, and a
 // single score buffer beside two of weights, were 4-6 % slower. Rates: 770 TFLOP/s for 256 lanes of int4, 460 for a 16-row

@@ -61,7 +61,7 @@ __device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
 // step of one, so that four of them stay finite.
 // Error of this form, in units of cap * 2^-23, from the sum of its roundings with q = 1 / (e^2u + 1) <= 1: the exponent's six
 // (its scale and products) 2 * 0.67, ex2 (2^-22) and the sum with one 2 * (0.5 + 0.5), the reciprocal (2^-23) and four products
-// 2 * 3, the last multiply-add 0.5: under 10, cap * 2^-19.7 (the worst of 16 million scores was cap * 2^-21.0 in a replay with
+// 2 * 3, the last multiply-add 0.5: under 10, cap * 2^-19.7 (the worst of 80 million scores was cap * 2^-20.8 in a replay with
 // exact ex2 and rcp). Caps up to 64 take it: under 2^-13 on a score, a quarter of what rounding the weights to 11 bits allows.
 // Beyond, scores are small against the cap and the difference from one loses them: below |u| = 1/4 the odd series u (1 - u^2/3 +
 // 2u^4/15 - 17u^6/315 + 62u^8/2835), whose next term is under 10^-8 there, takes over, and the result is good to about 10^-6 of

@@ -8,8 +8,9 @@
 //
 // The kernel is the row-tile kernel (row_tile.cuh) with rows gathered from many lanes. Measured, streaming kernel and merge
 // included: int4, 256 lanes over one 32K prefix 272 us (770 TFLOP/s; 1 364 us lane by lane), 32 over 8K 52 us (61), four over
-// 2K tokens of int8 25 us (20): three launches cost more than four short lanes' pages do. The crossover is near 200 MB of
-// pages saved.
+// 2K tokens of int8 25 us (20): three launches cost more than four short lanes' pages do. A tile takes the same time however many of
+// its rows are real, so small groups lose at any length (32 groups of four over 8K, int4: 176 us, 148 lane by lane); session.py has
+// the rule.
 #include "common.cuh"
 #include "decode_partials.cuh"
 #include "row_tile.cuh"

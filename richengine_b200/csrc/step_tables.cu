@@ -32,10 +32,12 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t value, uint32_t *scratch)
   return total;
 }
 
-// One block per lane: the lane is refused as a whole (its parameter blocks say so), so one block has to see all of its
-// page ids before it writes them. Bound by memory where tables are built anew (4 bytes in, 8 out per page), by latency
-// where only the pages behind `known_pages` are. 256 threads: eight blocks of an SM hold the largest batch in one wave.
-// Measured: 2.4 us for 8 lanes whose pages but one are known, 11 for 1 024 of 2 500 (31 MB, 2.8 TB/s: one wave that starts, streams and ends).
+// One block per lane. Entries are written as their ids are read; what waits for all of a lane's ids is the verdict on it (its
+// parameter blocks, slots and the status word), which one block gives without a counter of blocks that have arrived. Bound by
+// latency: where only the pages behind `known_pages` are new, one chain of dependent loads; where tables are built anew (4 bytes in,
+// 8 out per page), two rounds of 4-byte loads and 8-byte stores a thread, with a division by the extent's size per id. 256
+// threads: eight blocks of an SM hold the largest batch in one wave. Measured: 2.4 us for 8 lanes whose pages but one are known,
+// 11 for 1 024 of 2 500 (31 MB, 2.8 TB/s).
 __global__ void __launch_bounds__(kTableThreads)
 step_tables_kernel(const __grid_constant__ StepArgs a) {
   __shared__ uint32_t scratch[kTableThreads / 32];

@@ -1,5 +1,6 @@
-// window_tile.cuh — what the tcgen05 attention kernels share (verify_attention.cu, shared_prefix.cu): the roles' sizes, the
-// stored formats as 16-bit tensor-core operands, and the mbarrier, TMA, tcgen05 and tensor-memory primitives.
+// window_tile.cuh — what the tcgen05 attention kernels share (verify_attention.cu and row_tile.cuh, with shaped_attention.cu and
+// shared_prefix.cu on it): the roles' sizes, the stored formats as 16-bit tensor-core operands, and the mbarrier, TMA, tcgen05 and
+// tensor-memory primitives.
 #pragma once
 
 #include "common.cuh"

@@ -315,8 +315,8 @@ def _int32_vector(name: str, vector, size: int | None, device) -> None:
 class StepTables:
     """A step's page tables, parameter blocks and row slots, built on the GPU from request lengths (rk_step_tables).
 
-    `window`, `extent_stride`, `extent_pages` and `page_count` say where page ids lie (for_storage takes them from a
-    PageStorage); build() fills `entries`, `chunk_params`, `verify_params`, `row_offsets` and `row_slots` in stream order, and the
+    `window` (its base), `extent_stride`, `extent_pages` and `page_count` say where page ids lie (for_storage takes them from a
+    PageStorage; others answer for the whole pool lying in the window that attention is given); build() fills `entries`, `chunk_params`, `verify_params`, `row_offsets` and `row_slots` in stream order, and the
     stores and attention kernels take `table_pointers` and the parameter blocks as they are."""
 
     def __init__(self, lanes: int, table_pages: int, window: tuple[int, int], extent_stride: int, extent_pages: int,
