@@ -427,3 +427,21 @@ def test_a_captured_search_decides_on_the_gpu():
     del graph
     session.close()
     s.batch.close()
+
+
+def test_a_search_on_any_kind_of_stream():
+    """share_prefixes takes a stream as the other calls do: none, an object or a handle, the default stream's among them."""
+    s = Shared(INT4, [(6, 9)], 2, suffix=20)
+    session, params, attend = session_of(s)
+    side = torch.cuda.Stream()
+    for stream in (None, side, side.cuda_stream, torch.cuda.default_stream().cuda_stream):
+        torch.cuda.synchronize()
+        session.forget_prefixes()
+        session.share_prefixes(s.batch.pointers, params, minimum_pages=2, stream=stream)
+        torch.cuda.synchronize()
+        assert int(session._group_pages.max()) == 6 and int((session._lane_groups >= 0).sum()) == 9
+        got16, launches = attend()
+        assert launches == 3
+        check16(s, got16, (0, 10))
+    session.close()
+    s.batch.close()
